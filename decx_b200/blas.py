@@ -1,4 +1,4 @@
-"""Device-tensor front ends of the matrix-vector product, transpose and cast entry points of the C ABI
+"""Device-tensor front ends of the matrix-vector product, transpose, cast and row-norm entry points of the C ABI
 (used by the tests and the benchmark; torch only owns memory and the stream).
 
 Reference semantics: the Vector overloads of ``de::blas::cuda::GEMM`` (srcs/modules/BLAS/GEMM/CUDA/VMM.cu:142-184),
@@ -74,6 +74,130 @@ def cast(src, dtype, out=None):
     with torch.cuda.device(src.device):
         capi.check(capi.lib.decxb200_cast2d(kind, torch.cuda.current_stream().cuda_stream, rows, cols, src.data_ptr(),
                                             _ld(src), out.data_ptr(), _ld(out)))
+    return out
+
+
+_Q8_IN = {torch.float16: capi.FP16, torch.float32: capi.FP32}
+
+
+def new_q8(rows, cols, device):
+    """An empty 8-bit operand: a rows x cols float8_e4m3fn view whose rows start a multiple of 128 bytes apart
+    (the layout ``gemm.gemm_q8`` takes), and its rows' float32 scales."""
+    buf = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.float8_e4m3fn, device=device)
+    return buf[:, :cols], torch.empty(rows, dtype=torch.float32, device=device)
+
+
+def _q8_out(src, out, scales):
+    if out is None or scales is None:
+        q, s = new_q8(src.shape[0], src.shape[1], src.device)
+        out, scales = (q if out is None else out), (s if scales is None else scales)
+    if out.dtype != torch.float8_e4m3fn or out.shape != src.shape or out.device != src.device:
+        raise ValueError("out must be a float8_e4m3fn matrix of the input's shape on its device")
+    if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != src.shape[0] or not scales.is_contiguous() \
+            or scales.device != src.device:
+        raise ValueError("scales must be a contiguous float32 vector with one entry per row")
+    return out, scales
+
+
+def cast_q8(src, out=None, scales=None):
+    """``src`` (rows x cols, float16 or float32, pitched) as an 8-bit operand: returns ``(q, scales)`` with
+    ``scales[r] = max|src[r]| / 448`` and ``q = e4m3(src / scales[:, None])``.  Launches on torch's current stream."""
+    if not src.is_cuda:
+        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
+    dt = _Q8_IN.get(src.dtype)
+    if dt is None:
+        raise TypeError("cast_q8 takes float16 or float32")
+    lds = _ld(src)
+    out, scales = _q8_out(src, out, scales)
+    with torch.cuda.device(src.device):
+        capi.check(capi.lib.decxb200_cast_q8(dt, torch.cuda.current_stream().cuda_stream, src.shape[0], src.shape[1],
+                                             src.data_ptr(), lds, out.data_ptr(), _ld(out), scales.data_ptr()))
+    return out, scales
+
+
+def rmsnorm_q8(x, weight, residual=None, eps=1e-6, out=None, scales=None, sum_out=None):
+    """Root-mean-square norm of the rows of ``x + residual`` as an 8-bit operand: returns ``(q, scales, sum)``.
+
+    ``h = x + residual``, ``sum = h`` rounded to x's type (None without a residual), ``y = h / sqrt(mean(h^2) + eps) *
+    weight``, ``scales[r] = max|y[r]| / 448``, ``q = e4m3(y / scales[:, None])``.  float16 or float32, pitched rows;
+    ``sum_out`` may be ``x`` or ``residual`` themselves.  Launches on torch's current stream."""
+    if not x.is_cuda:
+        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
+    dt = _Q8_IN.get(x.dtype)
+    if dt is None or weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+        raise TypeError("x, weight and residual must share one dtype out of float16, float32")
+    ldx = _ld(x)
+    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or not weight.is_contiguous() or weight.device != x.device:
+        raise ValueError("weight must be a contiguous vector with one entry per column of x")
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError("sum_out without a residual")
+    else:
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ValueError("residual must have the shape of x")
+        if sum_out is None:
+            sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != x.device:
+            raise ValueError("sum_out must have the shape and type of x")
+    out, scales = _q8_out(x, out, scales)
+    with torch.cuda.device(x.device):
+        capi.check(capi.lib.decxb200_rmsnorm_q8(
+            dt, torch.cuda.current_stream().cuda_stream, x.shape[0], x.shape[1], x.data_ptr(), ldx,
+            residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
+            sum_out.data_ptr() if sum_out is not None else None, _ld(sum_out) if sum_out is not None else 0,
+            weight.data_ptr(), eps, out.data_ptr(), _ld(out), scales.data_ptr()))
+    return out, scales, sum_out
+
+
+def pack_q4(q):
+    """Values 0..15 (rows x cols, any integer type) in the layout ``gemv_q4`` takes: two per byte, the even column in the
+    low nibble, rows 16 bytes apart or a multiple.  Meant for laying weights out once."""
+    rows, cols = q.shape
+    buf = torch.zeros((rows, -(-cols // 32) * 16), dtype=torch.uint8, device=q.device)
+    nibbles = q.to(torch.uint8) & 15
+    buf[:, :(cols + 1) // 2] = nibbles[:, 0::2]
+    buf[:, :cols // 2] |= nibbles[:, 1::2] << 4
+    return buf[:, :(cols + 1) // 2]
+
+
+def gemv_q4(W, scales, x, group, zeros=None, x_scales=None, out_dtype=torch.float32, out=None):
+    """``y = W4 @ x`` for one vector (x of shape (cols,)) or 1 to 16 of them (x of shape (n, cols), y of shape (n, rows)).
+
+    ``W``: uint8, rows x ceil(cols / 2), two weights per byte (``pack_q4``); weight k of row r stands for
+    ``(q - zeros[r, k // group]) * scales[r, k // group]``, with 8 for the zero when ``zeros`` is None.  ``scales``:
+    float16; ``zeros``: uint8; ``group``: 32, 64 or 128.  ``x``: float16, or float8_e4m3fn whose rows stand for
+    ``x * x_scales[:, None]``.  Sums are float32.  Launches on torch's current stream."""
+    if not W.is_cuda:
+        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
+    if W.dtype != torch.uint8 or scales.dtype != torch.float16 or (zeros is not None and zeros.dtype != torch.uint8):
+        raise TypeError("gemv_q4 takes uint8 W, float16 scales and uint8 zeros")
+    xt = {torch.float16: capi.FP16, torch.float8_e4m3fn: capi.E4M3}.get(x.dtype)
+    if xt is None:
+        raise TypeError("x must be float16 or float8_e4m3fn")
+    single = x.dim() == 1
+    xm = x[None] if single else x
+    ldx, ldw, lds = _ld(xm), _ld(W), _ld(scales)
+    n, cols = xm.shape
+    rows = W.shape[0]
+    groups = -(-cols // group) if group > 0 else 0
+    if W.shape[1] != (cols + 1) // 2 or scales.shape != (rows, groups) or (zeros is not None and zeros.shape != (rows, groups)):
+        raise ValueError("W is rows x ceil(cols / 2), scales and zeros rows x ceil(cols / group), x vectors of cols entries")
+    if x_scales is not None and (x_scales.dtype != torch.float32 or x_scales.numel() != n or not x_scales.is_contiguous()):
+        raise ValueError("x_scales must be contiguous float32 with one entry per vector")
+    if out is None:
+        out = torch.empty(rows if single else (n, rows), dtype=out_dtype, device=W.device)
+    yt = {torch.float16: capi.FP16, torch.float32: capi.FP32}.get(out.dtype)
+    ym = out[None] if single else out
+    if yt is None or ym.shape != (n, rows):
+        raise ValueError("the result is float16 or float32, one entry per row of W for each vector")
+    dev = W.device
+    if any(a is not None and a.device != dev for a in (scales, zeros, x, x_scales, out)):
+        raise ValueError("all operands must be on one device")
+    with torch.cuda.device(dev):
+        capi.check(capi.lib.decxb200_gemv_q4(
+            xt, yt, torch.cuda.current_stream().cuda_stream, rows, cols, n, group, W.data_ptr(), ldw, scales.data_ptr(), lds,
+            zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else 0, xm.data_ptr(), ldx,
+            x_scales.data_ptr() if x_scales is not None else None, ym.data_ptr(), _ld(ym)))
     return out
 
 

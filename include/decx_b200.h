@@ -33,6 +33,7 @@ extern "C" {
 #define DECXB200_FP16 3
 #define DECXB200_CPLXF 5
 #define DECXB200_CPLXD 6
+#define DECXB200_E4M3 32           /* 8-bit float of quantised operands; no de:: type has this value */
 
 #define DECXB200_EINVAL (-1)       /* null pointer, zero extent, unknown dtype            */
 #define DECXB200_EALIGN (-2)       /* fp16 operand pitch/base not 16-byte aligned (TMA)    */
@@ -225,6 +226,51 @@ DECXB200_API int decxb200_transpose(int elem_bytes, void* stream, uint32_t rows,
 #define DECXB200_CAST_F32_I32 5
 DECXB200_API int decxb200_cast2d(int kind, void* stream, uint32_t rows, uint32_t cols,
                                  const void* src, uint64_t lds, void* dst, uint64_t ldd);
+
+/*
+ * 8-bit operands.  A quantised operand is a pitched rows x cols matrix q of e4m3 bytes (1 sign, 4 exponent, 3 mantissa
+ * bits; largest value 448, no infinity) with one fp32 scale per row; it stands for q * scale[row].  The three entry
+ * points below have no counterpart in the reference, whose narrowest type is fp16; they extend its type casts and its
+ * GEMM by the operand type of quantised linear layers.
+ *
+ * decxb200_cast_q8:     y = src
+ * decxb200_rmsnorm_q8:  h = x + residual;  sum = h rounded to dtype;  y = h * rsqrt(mean of h^2 over the row + eps) * weight
+ *     scales[row] = max|y| / 448,   q = e4m3(y / scales[row]), nearest even
+ *
+ *   dtype: DECXB200_FP16 or DECXB200_FP32, the type of x / src, residual, sum and weight.  All arithmetic is fp32; the
+ *   norm sees h before it is rounded.  residual == NULL: nothing is added (sum must then be NULL); sum == NULL: the sum
+ *   is not stored.  sum may be x or residual (the same pointer and pitch); otherwise inputs and outputs may not overlap.
+ *   weight: cols elements.  eps: a positive normal fp32 number.
+ *   A row of zeros has scale 0 and q 0.  A row that holds a NaN or an infinity, or whose sum of squares exceeds the
+ *   fp32 range, gets NaN for its scale and for every q.
+ *   Any alignment and pitch works; 16-byte aligned bases (8-byte for q) and pitches are faster, and q needs a 16-byte
+ *   aligned base and a pitch that is a multiple of 16 to be an operand of decxb200_gemm_q8.  Asynchronous on `stream`.
+ */
+DECXB200_API int decxb200_cast_q8(int dtype, void* stream, uint32_t rows, uint32_t cols, const void* src, uint64_t lds,
+                                  void* q, uint64_t ldq, float* scales);
+DECXB200_API int decxb200_rmsnorm_q8(int dtype, void* stream, uint32_t rows, uint32_t cols, const void* x, uint64_t ldx,
+                                     const void* residual, uint64_t ldr, void* sum, uint64_t ldsum, const void* weight,
+                                     float eps, void* q, uint64_t ldq, float* scales);
+
+/*
+ * Matrix-vector products with 4-bit weights, for 1 to 16 vectors at once (no counterpart in the reference; the 4-bit
+ * sibling of decxb200_gemv's Matrix x Vector form):
+ *   y[v][r] = x_scales[v] * sum_k (q[r][k] - z[r][k / group]) * scales[r][k / group] * x[v][k]
+ *   W:       rows x cols 4-bit weights q, two per byte: byte k / 2 of a row holds column k in its low nibble when k is
+ *            even, in its high nibble when it is odd.  ldw BYTES per row, a multiple of 16; base 16-byte aligned.  The
+ *            unused nibble of an odd row length may hold anything.
+ *   scales:  rows x ceil(cols / group) fp16, ld_scales elements per row.  group: 32, 64 or 128 consecutive columns.
+ *   zeros:   rows x ceil(cols / group) uint8 zero points, ld_zeros elements per row; NULL: z = 8.
+ *   x:       n_vec x cols, fp16 or e4m3 (x_dtype DECXB200_FP16 / DECXB200_E4M3), ldx elements per vector.
+ *   x_scales: n_vec fp32 factors (the scales of an 8-bit operand), or NULL: 1.
+ *   y:       n_vec x rows, fp16 or fp32 (y_dtype), ldy elements per vector.
+ * q - z times x is exact, sums and scales are fp32; an fp16 y is rounded once.  The weights are read once whatever
+ * n_vec is.  Partial sums are added in a fixed order: results do not depend on timing.  Asynchronous on `stream`.
+ */
+DECXB200_API int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint32_t cols, uint32_t n_vec,
+                                  uint32_t group, const void* W, uint64_t ldw, const void* scales, uint64_t ld_scales,
+                                  const void* zeros, uint64_t ld_zeros, const void* x, uint64_t ldx,
+                                  const float* x_scales, void* y, uint64_t ldy);
 
 /*
  * fp32 2-D convolution as im2col + one 3xTF32 GEMM: the consumer of the GEMM core in DECX's NN module
