@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import capi
-from .gemm import _ld
+from .gemm import _ld, _on, _stream
 
 _OUT = {(capi.FP32, 0): torch.float32, (capi.FP16, capi.ACCU_L1): torch.float32,
         (capi.FP16, capi.ACCU_L2): torch.float16, (capi.FP16, capi.ACCU_L3): torch.float16}
@@ -109,9 +109,10 @@ def cast_q8(src, out=None, scales=None):
         raise TypeError("cast_q8 takes float16 or float32")
     lds = _ld(src)
     out, scales = _q8_out(src, out, scales)
-    with torch.cuda.device(src.device):
-        capi.check(capi.lib.decxb200_cast_q8(dt, torch.cuda.current_stream().cuda_stream, src.shape[0], src.shape[1],
-                                             src.data_ptr(), lds, out.data_ptr(), _ld(out), scales.data_ptr()))
+    dev = src.device
+    rows, cols = src.shape
+    _on(dev, capi.lib.decxb200_cast_q8, dt, _stream(dev), rows, cols, src.data_ptr(), lds, out.data_ptr(), _ld(out),
+        scales.data_ptr())
     return out, scales
 
 
@@ -126,26 +127,25 @@ def rmsnorm_q8(x, weight, residual=None, eps=1e-6, out=None, scales=None, sum_ou
     dt = _Q8_IN.get(x.dtype)
     if dt is None or weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
         raise TypeError("x, weight and residual must share one dtype out of float16, float32")
-    ldx = _ld(x)
-    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or not weight.is_contiguous() or weight.device != x.device:
+    ldx, dev = _ld(x), x.device
+    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or not weight.is_contiguous() or weight.device != dev:
         raise ValueError("weight must be a contiguous vector with one entry per column of x")
     if residual is None:
         if sum_out is not None:
             raise ValueError("sum_out without a residual")
     else:
-        if residual.shape != x.shape or residual.device != x.device:
+        if residual.shape != x.shape or residual.device != dev:
             raise ValueError("residual must have the shape of x")
         if sum_out is None:
             sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != x.device:
+        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != dev:
             raise ValueError("sum_out must have the shape and type of x")
     out, scales = _q8_out(x, out, scales)
-    with torch.cuda.device(x.device):
-        capi.check(capi.lib.decxb200_rmsnorm_q8(
-            dt, torch.cuda.current_stream().cuda_stream, x.shape[0], x.shape[1], x.data_ptr(), ldx,
-            residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
-            sum_out.data_ptr() if sum_out is not None else None, _ld(sum_out) if sum_out is not None else 0,
-            weight.data_ptr(), eps, out.data_ptr(), _ld(out), scales.data_ptr()))
+    rows, cols = x.shape
+    _on(dev, capi.lib.decxb200_rmsnorm_q8, dt, _stream(dev), rows, cols, x.data_ptr(), ldx,
+        residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
+        sum_out.data_ptr() if sum_out is not None else None, _ld(sum_out) if sum_out is not None else 0,
+        weight.data_ptr(), eps, out.data_ptr(), _ld(out), scales.data_ptr())
     return out, scales, sum_out
 
 
@@ -193,11 +193,9 @@ def gemv_q4(W, scales, x, group, zeros=None, x_scales=None, out_dtype=torch.floa
     dev = W.device
     if any(a is not None and a.device != dev for a in (scales, zeros, x, x_scales, out)):
         raise ValueError("all operands must be on one device")
-    with torch.cuda.device(dev):
-        capi.check(capi.lib.decxb200_gemv_q4(
-            xt, yt, torch.cuda.current_stream().cuda_stream, rows, cols, n, group, W.data_ptr(), ldw, scales.data_ptr(), lds,
-            zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else 0, xm.data_ptr(), ldx,
-            x_scales.data_ptr() if x_scales is not None else None, ym.data_ptr(), _ld(ym)))
+    _on(dev, capi.lib.decxb200_gemv_q4, xt, yt, _stream(dev), rows, cols, n, group, W.data_ptr(), ldw, scales.data_ptr(), lds,
+        zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else 0, xm.data_ptr(), ldx,
+        x_scales.data_ptr() if x_scales is not None else None, ym.data_ptr(), _ld(ym))
     return out
 
 

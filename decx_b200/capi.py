@@ -9,6 +9,7 @@ import os
 
 FP32, FP64, FP16, CPLXF, CPLXD = 1, 2, 3, 5, 6
 E4M3 = 32
+TILE_AUTO, TILE_Q8_THIN, TILE_Q8_PAIR = 0, 1, 2
 ACCU_L1, ACCU_L2, ACCU_L3 = 0, 1, 2
 CAST_F32_F16, CAST_F16_F32, CAST_F32_F64, CAST_F64_F32, CAST_I32_F32, CAST_F32_I32 = range(6)
 
@@ -89,6 +90,9 @@ def _load():
     lib.decxb200_cast_q8.argtypes = [ci, vp, u32, u32, vp, u64, vp, u64, vp]
     lib.decxb200_rmsnorm_q8.restype = ci
     lib.decxb200_rmsnorm_q8.argtypes = [ci, vp, u32, u32, vp, u64, vp, u64, vp, u64, vp, f32, vp, u64, vp]
+    pf32 = ctypes.POINTER(ctypes.c_float)
+    lib.decxb200_gemm_q8.restype = ci
+    lib.decxb200_gemm_q8.argtypes = [ci, vp, u32, u32, u32, vp, u64, vp, vp, u64, vp, vp, u64, vp, u64, pf32, pf32, vp, ci]
     lib.decxb200_gemv_q4.restype = ci
     lib.decxb200_gemv_q4.argtypes = [ci, ci, vp, u32, u32, u32, u32, vp, u64, vp, u64, vp, u64, vp, u64, vp, vp, u64]
     lib.decxb200_conv2d_fp32_out_dims.restype = ci
@@ -135,7 +139,7 @@ EXPORTS = [
     "decxb200_gemm_host_arena_bytes", "decxb200_gemm_host", "decxb200_gemm_host_multi_arena_bytes", "decxb200_gemm_host_multi_plan",
     "decxb200_gemm_host_multi",
     "decxb200_gemm_fp32_noalloc", "decxb200_gemv_workspace_bytes", "decxb200_gemv", "decxb200_transpose",
-    "decxb200_cast2d", "decxb200_cast_q8", "decxb200_rmsnorm_q8", "decxb200_gemv_q4", "decxb200_conv2d_fp32_out_dims", "decxb200_conv2d_fp32_workspace_bytes", "decxb200_conv2d_fp32",
+    "decxb200_cast2d", "decxb200_cast_q8", "decxb200_rmsnorm_q8", "decxb200_gemm_q8", "decxb200_gemv_q4", "decxb200_conv2d_fp32_out_dims", "decxb200_conv2d_fp32_workspace_bytes", "decxb200_conv2d_fp32",
     "decxb200_gemm_fp16_panels", "decxb200_fetch_scratch_bytes", "decxb200_gemm_fp16_fetch", "decxb200_gemm_fp16_fetch_staged", "decxb200_fetch_d_stage_bytes", "decxb200_copy2d_async", "decxb200_write_flag_async",
     "decxb200_ipc_alloc", "decxb200_ipc_free", "decxb200_ipc_export", "decxb200_ipc_open", "decxb200_ipc_close",
     "decxb200_last_launch_count", "decxb200_last_kernel_variant", "decxb200_tensor_map_cache_stats", "decxb200_debug_stats", "decxb200_strerror", "decxb200_version",

@@ -106,6 +106,40 @@ int make_map(CUtensorMap* map, bool f16, const void* base, uint64_t rows, uint64
     return r == CUDA_SUCCESS ? 0 : DECXB200_EDRIVER;
 }
 
+}  // namespace
+
+// The same for another translation unit, by element size: 1 = bytes, 2 = fp16, 4 = fp32.
+int dxb_host::tensor_map_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                            uint32_t box_cols, uint32_t box_rows) {
+    if (elem_bytes != 1) return make_map(map, elem_bytes == 2, base, rows, cols, ld, box_cols, box_rows);
+    const MapKey mk = {base, rows, cols, ld, box_cols, box_rows, 0, 2, int(CU_TENSOR_MAP_SWIZZLE_128B), 2};
+    if (const CUtensorMap* hit = t_maps.find(mk)) { *map = *hit; ++t_map_hits; return 0; }
+    ++t_map_misses;
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (enc == nullptr) return DECXB200_EDRIVER;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld};
+    cuuint32_t box[2] = {box_cols, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) t_maps.put(mk, *map);
+    return r == CUDA_SUCCESS ? 0 : DECXB200_EDRIVER;
+}
+
+// every wait inside the kernels gives up after this long (DECXB200_WAIT_LIMIT_MS, default 4 s)
+unsigned long long dxb_host::wait_limit_ns() {
+    static const unsigned long long limit_ns = [] {
+        const char* e = getenv("DECXB200_WAIT_LIMIT_MS");
+        const long v = e ? atol(e) : 0;
+        return v > 0 ? (unsigned long long)v * 1000000ull : 4000000000ull;
+    }();
+    return limit_ns;
+}
+
+namespace {
+
 // B (K x N row-major) as a 3-D tensor (column-in-chunk, k, chunk): chunk c holds columns
 // [c*chunk_cols, (c+1)*chunk_cols), i.e. dimension 2 has a stride of 128 bytes.  A box of
 // (chunk_cols, box_k, box_chunks) then lands in shared memory exactly as box_chunks consecutive
@@ -363,13 +397,7 @@ void fill_common(GemmParams& p, const Scalars& sc, const void* C, void* D, unsig
         void* addr = nullptr;
         if (cudaGetSymbolAddress(&addr, g_debug_stats) == cudaSuccess) p.stats = static_cast<unsigned long long*>(addr);
     }
-    // every wait inside the kernels gives up after this long (DECXB200_WAIT_LIMIT_MS, default 4 s)
-    static const unsigned long long limit_ns = [] {
-        const char* e = getenv("DECXB200_WAIT_LIMIT_MS");
-        const long v = e ? atol(e) : 0;
-        return v > 0 ? (unsigned long long)v * 1000000ull : 4000000000ull;
-    }();
-    p.wait_limit_ns = limit_ns;
+    p.wait_limit_ns = dxb_host::wait_limit_ns();
     p.alpha_re = sc.ar;
     p.alpha_im = sc.ai;
     p.beta_re = sc.br;
@@ -1166,7 +1194,8 @@ const char* decxb200_strerror(int code) {
     switch (code) {
         case 0: return "success";
         case DECXB200_EINVAL: return "invalid argument (null pointer, zero extent, pitch smaller than width, unknown dtype)";
-        case DECXB200_EALIGN: return "fp16 operands need 16-byte aligned base addresses and pitches that are multiples of 8 elements";
+        case DECXB200_EALIGN: return "fp16 operands need 16-byte aligned base addresses and pitches that are multiples of 8 elements "
+                                     "(8-bit and 4-bit operands: pitches of a multiple of 16 bytes; other arrays: the alignment of their elements)";
         case DECXB200_EWORKSPACE: return "workspace is missing, not 256-byte aligned, or smaller than decxb200_gemm_workspace_bytes()";
         case DECXB200_EDRIVER: return "cuTensorMapEncodeTiled is unavailable or rejected the tensor (no CUDA driver / no sm_100 device?)";
         case DECXB200_ETOOLARGE: return "problem extent beyond what this entry point supports";

@@ -5,6 +5,7 @@
 
 #include "../../include/decx_b200.h"
 #include "capi_shared.h"
+#include "gemm_q8.cuh"
 #include "gemv_q4.cuh"
 #include "rownorm_q8.cuh"
 
@@ -65,6 +66,27 @@ int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
     return 0;
 }
 
+template <typename K, typename... Args>
+int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) return int(e);
+    dxb_host::count_launch();
+    return 0;
+}
+
 constexpr uint32_t Q4_MAX_VEC = 16, Q4_MAX_RANKS = 8;
 
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
@@ -75,23 +97,7 @@ int launch_gemv_q4(cudaStream_t s, const GemvQ4Params& p) {
     if (rc != 0) return rc;
     const uint64_t blocks = (uint64_t(p.rows) + Q4_ROWS - 1) / Q4_ROWS * p.ranks;
     if (blocks > 0x7fffffffull) return DECXB200_ETOOLARGE;
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(unsigned(blocks));
-    cfg.blockDim = dim3(Q4_THREADS);
-    cfg.dynamicSmemBytes = q4_smem_bytes(p.slice, GROUP, NT, p.n_vec, ZEROS);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.ranks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e != cudaSuccess) return int(e);
-    dxb_host::count_launch();
-    return 0;
+    return launch_cluster(kern, unsigned(blocks), Q4_THREADS, q4_smem_bytes(p.slice, GROUP, NT, p.n_vec, ZEROS), p.ranks, s, p);
 }
 
 template <int GROUP, int NT, bool ZEROS>
@@ -106,9 +112,106 @@ int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) 
     return z ? run_gemv_q4<GROUP, 1, true>(s, x8, f32, p) : run_gemv_q4<GROUP, 1, false>(s, x8, f32, p);
 }
 
+// ------------------------------------------------------------------------------------------------ 8-bit GEMM
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n;
+}
+
+template <int BN, typename T>
+int launch_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
+    using Cfg = ThinCfg<BN>;
+    CUtensorMap ma, mb;
+    int rc;
+    if ((rc = dxb_host::tensor_map_2d(&ma, 1, A, p.M, p.K, lda, Q8_KB, BN)) != 0) return rc;
+    if ((rc = dxb_host::tensor_map_2d(&mb, 1, B, p.N, p.K, ldb, Q8_KB, 128)) != 0) return rc;
+    auto kern = gemm_q8_thin_kernel<BN, T>;
+    static std::atomic<uint64_t> done{0};
+    if ((rc = allow_smem(kern, Cfg::SMEM_BYTES, done)) != 0) return rc;
+    p.tiles_m = (p.M + BN - 1) / BN;
+    p.tiles_n = (p.N + 127) / 128;
+    const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
+    const uint32_t n_kb = (p.K + Q8_KB - 1) / Q8_KB;
+    p.ranks = 1;
+    while (p.ranks < 8 && tiles * p.ranks * 2 <= 296 && n_kb >= p.ranks * 2 * 4) p.ranks *= 2;
+    if (tiles * p.ranks > 0x7fffffffull) return DECXB200_ETOOLARGE;
+    return launch_cluster(kern, unsigned(tiles * p.ranks), 192, Cfg::SMEM_BYTES, p.ranks, s, ma, mb, p);
+}
+
+template <typename T>
+int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
+    CUtensorMap ma, mb, md, mc;
+    int rc;
+    if ((rc = dxb_host::tensor_map_2d(&ma, 1, A, p.M, p.K, lda, Q8_KB, 128)) != 0) return rc;
+    if ((rc = dxb_host::tensor_map_2d(&mb, 1, B, p.N, p.K, ldb, Q8_KB, 128)) != 0) return rc;
+    md = mc = ma;
+    const uint64_t e = sizeof(T);
+    if (aligned16(p.D) && (p.ldd * e) % 16 == 0 &&
+        dxb_host::tensor_map_2d(&md, int(e), p.D, p.M, p.N, p.ldd, uint32_t(128 / e), 32) == 0)
+        p.d_tma = 1;
+    if (p.d_tma && p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0 &&
+        dxb_host::tensor_map_2d(&mc, int(e), p.C, p.M, p.N, p.ldc, uint32_t(128 / e), 32) == 0)
+        p.c_tma = 1;
+    auto kern = gemm_q8_pair_kernel<T>;
+    static std::atomic<uint64_t> done{0};
+    if ((rc = allow_smem(kern, PairCfg::SMEM_BYTES, done)) != 0) return rc;
+    p.tiles_m = uint32_t((uint64_t(p.M) + 255) / 256);
+    p.tiles_n = uint32_t((uint64_t(p.N) + 255) / 256);
+    const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
+    if (tiles > 0x7fffffffull) return DECXB200_ETOOLARGE;
+    p.group_m = p.tiles_m < 8 ? p.tiles_m : 8;
+    uint64_t pairs = uint64_t(sm_count()) / 2;
+    if (pairs > tiles) pairs = tiles;
+    if (pairs == 0) pairs = 1;
+    return launch_cluster(kern, unsigned(2 * pairs), PairCfg::THREADS, PairCfg::SMEM_BYTES, 2, s, ma, mb, md, mc, p);
+}
+
+template <typename T>
+int run_gemm_q8(cudaStream_t s, const GemmQ8Params& p, const void* A, uint64_t lda, const void* B, uint64_t ldb, int tile) {
+    if (tile == DECXB200_TILE_AUTO) {
+        const uint64_t tiles = (uint64_t(p.M) + 255) / 256 * ((uint64_t(p.N) + 255) / 256);
+        tile = p.M > 128 && tiles >= 48 ? DECXB200_TILE_Q8_PAIR : DECXB200_TILE_Q8_THIN;
+    }
+    if (tile == DECXB200_TILE_Q8_PAIR) return launch_q8_pair<T>(s, p, A, lda, B, ldb);
+    if (p.M <= 16) return launch_q8_thin<16, T>(s, p, A, lda, B, ldb);
+    if (p.M <= 32) return launch_q8_thin<32, T>(s, p, A, lda, B, ldb);
+    if (p.M <= 64) return launch_q8_thin<64, T>(s, p, A, lda, B, ldb);
+    return launch_q8_thin<128, T>(s, p, A, lda, B, ldb);
+}
+
 }  // namespace
 
 extern "C" {
+
+int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_t N, uint32_t K, const void* A, uint64_t lda,
+                     const float* a_scales, const void* B, uint64_t ldb, const float* b_scales, const void* C, uint64_t ldc,
+                     void* D, uint64_t ldd, const float* alpha, const float* beta, unsigned* status, int tile) {
+    dxb_host::reset_launches();
+    if (d_dtype != DECXB200_FP16 && d_dtype != DECXB200_FP32) return DECXB200_EINVAL;
+    if (A == nullptr || B == nullptr || D == nullptr || a_scales == nullptr || b_scales == nullptr) return DECXB200_EINVAL;
+    if (M == 0 || N == 0 || K == 0 || lda < K || ldb < K || ldd < N || (C != nullptr && ldc < N)) return DECXB200_EINVAL;
+    if (tile != DECXB200_TILE_AUTO && tile != DECXB200_TILE_Q8_THIN && tile != DECXB200_TILE_Q8_PAIR) return DECXB200_EINVAL;
+    if (M > 0x7fffff00u || N > 0x7fffff00u || K > 0x7fffff00u) return DECXB200_ETOOLARGE;   // TMA coordinates are signed
+    if (!aligned16(A) || !aligned16(B) || (lda % 16) != 0 || (ldb % 16) != 0) return DECXB200_EALIGN;
+    const uintptr_t e = d_dtype == DECXB200_FP16 ? 2 : 4;
+    if ((reinterpret_cast<uintptr_t>(a_scales) & 3) != 0 || (reinterpret_cast<uintptr_t>(b_scales) & 3) != 0 ||
+        reinterpret_cast<uintptr_t>(C) % e != 0 || reinterpret_cast<uintptr_t>(D) % e != 0)
+        return DECXB200_EALIGN;
+    GemmQ8Params p;
+    memset(&p, 0, sizeof(p));
+    p.M = M; p.N = N; p.K = K;
+    p.sa = a_scales; p.sb = b_scales;
+    p.alpha = alpha != nullptr ? *alpha : 1.f;
+    p.beta = beta != nullptr ? *beta : 0.f;
+    p.C = p.beta != 0.f ? C : nullptr;
+    p.ldc = ldc;
+    p.D = D; p.ldd = ldd;
+    p.status = status;
+    p.wait_limit_ns = dxb_host::wait_limit_ns();
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return d_dtype == DECXB200_FP16 ? run_gemm_q8<__half>(s, p, A, lda, B, ldb, tile) : run_gemm_q8<float>(s, p, A, lda, B, ldb, tile);
+}
 
 int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint32_t cols, uint32_t n_vec, uint32_t group,
                      const void* W, uint64_t ldw, const void* scales, uint64_t ld_scales, const void* zeros,

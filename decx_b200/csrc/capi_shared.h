@@ -2,6 +2,7 @@
 #pragma once
 #include <cstddef>
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace dxb_host {
@@ -12,6 +13,13 @@ void reset_launches();
 
 inline uint64_t round_up(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Tensor map of a pitched rows x cols matrix with a box_cols x box_rows box, 128-byte swizzle, zero fill; elements of 1
+// (bytes), 2 (fp16) or 4 (fp32) bytes.  Cached per thread.
+int tensor_map_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                  uint32_t box_cols, uint32_t box_rows);
+// how long a wait inside a kernel may last before it reports through the status word
+unsigned long long wait_limit_ns();
 
 // fp64 / complex-fp64 GEMM on `stream` (real expansion of B in `workspace` for the complex case;
 // b_expanded: the workspace already holds it, e.g. from the previous row block of the same B)

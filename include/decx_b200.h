@@ -228,6 +228,25 @@ DECXB200_API int decxb200_cast2d(int kind, void* stream, uint32_t rows, uint32_t
                                  const void* src, uint64_t lds, void* dst, uint64_t ldd);
 
 /*
+ * 8-bit GEMM:  D = alpha * diag(a_scales) * A * B^T * diag(b_scales) + beta * C   (no counterpart in the reference).
+ *   A: M x K and B: N x K, e4m3, K innermost in both (B as a linear layer keeps its weights, one row per output), lda /
+ *   ldb bytes per row; a_scales: M, b_scales: N fp32 factors.  These are the operands decxb200_cast_q8 and
+ *   decxb200_rmsnorm_q8 write.  C, D: M x N of d_dtype (DECXB200_FP16 or DECXB200_FP32); C may be NULL, or D itself
+ *   with D's pitch.  alpha, beta: host pointers, NULL means 1 / 0; C is not read when beta == 0.
+ *   Sums are fp32; an fp16 D is rounded once.  tcgen05 kind::f8f6f4; one launch, no workspace, the same result every
+ *   time.  lda, ldb: multiples of 16, bases 16-byte aligned.  status as for decxb200_gemm.  Asynchronous on `stream`.
+ *   tile: DECXB200_TILE_AUTO, or one of the two kernels (tests and measurements): THIN cuts K over a cluster of CTAs
+ *   and is made for few rows of A, PAIR works on 256 x 256 tiles.
+ */
+#define DECXB200_TILE_Q8_THIN 1
+#define DECXB200_TILE_Q8_PAIR 2
+DECXB200_API int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_t N, uint32_t K,
+                                  const void* A, uint64_t lda, const float* a_scales,
+                                  const void* B, uint64_t ldb, const float* b_scales,
+                                  const void* C, uint64_t ldc, void* D, uint64_t ldd,
+                                  const float* alpha, const float* beta, unsigned* status, int tile);
+
+/*
  * 8-bit operands.  A quantised operand is a pitched rows x cols matrix q of e4m3 bytes (1 sign, 4 exponent, 3 mantissa
  * bits; largest value 448, no infinity) with one fp32 scale per row; it stands for q * scale[row].  The three entry
  * points below have no counterpart in the reference, whose narrowest type is fp16; they extend its type casts and its
