@@ -1,6 +1,7 @@
 // extern "C" layer, third part: the operators on 8-bit and 4-bit operands.  See include/decx_b200.h for the contracts.
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 
 #include "../../include/decx_b200.h"
@@ -20,10 +21,60 @@ inline int last_error() {
     return e == cudaSuccess ? 0 : int(e);
 }
 
+// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device.
+template <typename K>
+int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return int(e);
+    if (dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return int(e);
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return 0;
+}
+
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n;
+}
+
+template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
+int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
+    constexpr uint32_t U = 8 * sizeof(T) / 16 + (SHIFT ? 1 : 0);
+    const uint32_t row = threads * NCH * U * (RES ? 2 : 1) * 16;      // one slot of the ring
+    auto kern = row_q8_ring_kernel<T, NORM, RES, WARP, SHIFT, NCH>;
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> regs{0};
+    int rc = allow_smem(kern, 220 * 1024, done);
+    if (rc != 0) return rc;
+    int r = regs.load(std::memory_order_relaxed);
+    if (r == 0) {
+        cudaFuncAttributes a;
+        const cudaError_t e = cudaFuncGetAttributes(&a, kern);
+        if (e != cudaSuccess) return int(e);
+        regs.store(r = a.numRegs, std::memory_order_relaxed);
+    }
+    const uint32_t by_regs = 65536u / (uint32_t((r + 7) / 8 * 8) * threads), by_threads = 2048u / threads;
+    const uint32_t most = by_regs < by_threads ? by_regs : by_threads;
+    p.depth = 4;
+    auto fits = [&](uint32_t d) { return 225u * 1024 / (row * d + 2048); };
+    while (p.depth > 2 && fits(p.depth) < most) --p.depth;            // as many CTAs as registers and threads allow
+    while (p.depth < 4 && fits(p.depth) == 1 && row * (p.depth + 1) <= 220 * 1024) ++p.depth;
+    const uint32_t by_smem = fits(p.depth);
+    const uint32_t per_sm = by_smem < most ? by_smem : most;
+    const uint64_t want = WARP ? (uint64_t(p.rows) + threads / 32 - 1) / (threads / 32) : p.rows;
+    const uint64_t have = uint64_t(sm_count()) * (per_sm ? per_sm : 1);
+    kern<<<unsigned(want < have ? want : have), threads, row * p.depth, s>>>(p);
+    dxb_host::count_launch();
+    return last_error();
+}
+
+// kernels that keep one row per CTA or warp: few rows (no ring to fill), or operands that only single elements fit
 template <typename T, bool NORM, bool VEC>
 int launch_row_q8(cudaStream_t s, const RowQ8Params& p) {
     if (p.cols <= 1024) {
-        // a warp per row: eight rows share a CTA, no barrier
         const unsigned blocks = unsigned((uint64_t(p.rows) + 7) / 8);
         if (p.cols <= 256) row_q8_kernel<T, NORM, true, VEC, 1><<<blocks, 256, 0, s>>>(p);
         else if (p.cols <= 512) row_q8_kernel<T, NORM, true, VEC, 2><<<blocks, 256, 0, s>>>(p);
@@ -41,29 +92,32 @@ int launch_row_q8(cudaStream_t s, const RowQ8Params& p) {
     return last_error();
 }
 
+template <typename T, bool NORM, bool RES, bool SHIFT>
+int launch_row_q8_shape(cudaStream_t s, const RowQ8Params& p) {
+    if (p.cols <= 256) return launch_row_q8_ring<T, NORM, RES, true, SHIFT, 1>(s, p, 256);
+    if (p.cols <= 512) return launch_row_q8_ring<T, NORM, RES, true, SHIFT, 2>(s, p, 256);
+    if (p.cols <= 1024) return launch_row_q8_ring<T, NORM, RES, true, SHIFT, 4>(s, p, 256);
+    return launch_row_q8_ring<T, NORM, RES, false, SHIFT, 2>(s, p, (p.cols + 511) / 512 * 32);
+}
+
 template <typename T, bool NORM>
 int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     const uint64_t e = sizeof(T);
     auto elem = [&](const void* a) { return reinterpret_cast<uintptr_t>(a) % e == 0; };
     if (!elem(p.x) || !elem(p.r) || !elem(p.sum) || !elem(p.w) || (reinterpret_cast<uintptr_t>(p.scales) & 3) != 0)
         return DECXB200_EALIGN;
-    const bool vec = aligned16(p.x) && (p.ldx * e) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 &&
-                     (p.r == nullptr || (aligned16(p.r) && (p.ldr * e) % 16 == 0)) &&
-                     (p.sum == nullptr || (aligned16(p.sum) && (p.lds * e) % 16 == 0)) && aligned16(p.w);
-    return vec ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
-}
-
-// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device.
-template <typename K>
-int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return int(e);
-    if (dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return 0;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return int(e);
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
-    return 0;
+    const bool rows16 = aligned16(p.x) && (p.ldx * e) % 16 == 0 && (p.r == nullptr || (aligned16(p.r) && (p.ldr * e) % 16 == 0)) &&
+                        (p.sum == nullptr || (aligned16(p.sum) && (p.lds * e) % 16 == 0));
+    const bool out8 = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 && aligned16(p.w);
+    // two slots of the ring have to fit: the limit is 1024 threads times two pieces of 8, or shared memory
+    const uint64_t slot = uint64_t(p.cols + 511) / 512 * 512 * (e + (rows16 ? 0 : 2)) * (p.r != nullptr ? 2 : 1);
+    const bool ring = out8 && p.cols <= 16384 && 2 * slot <= 200 * 1024 && (p.rows > 296 || !rows16);
+    if (!ring) return rows16 && out8 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
+    if constexpr (NORM) {
+        if (p.r != nullptr)
+            return rows16 ? launch_row_q8_shape<T, true, true, false>(s, p) : launch_row_q8_shape<T, true, true, true>(s, p);
+    }
+    return rows16 ? launch_row_q8_shape<T, NORM, false, false>(s, p) : launch_row_q8_shape<T, NORM, false, true>(s, p);
 }
 
 template <typename K, typename... Args>
@@ -113,12 +167,6 @@ int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) 
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit GEMM
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-    return n;
-}
-
 template <int BN, typename T>
 int launch_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
     using Cfg = ThinCfg<BN>;
@@ -133,6 +181,7 @@ int launch_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
     p.tiles_n = (p.N + 127) / 128;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     const uint32_t n_kb = (p.K + Q8_KB - 1) / Q8_KB;
+    p.vec_d = (reinterpret_cast<uintptr_t>(p.D) % (4 * sizeof(T))) == 0 && p.ldd % 4 == 0;
     p.ranks = 1;
     while (p.ranks < 8 && tiles * p.ranks * 2 <= 296 && n_kb >= p.ranks * 2 * 4) p.ranks *= 2;
     if (tiles * p.ranks > 0x7fffffffull) return DECXB200_ETOOLARGE;
@@ -238,12 +287,15 @@ int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint
     p.x = x; p.ldx = ldx; p.xs = x_scales;
     p.y = y; p.ldy = ldy;
     p.rows = rows; p.cols = cols; p.n_vec = n_vec;
+    p.vec_s = (reinterpret_cast<uintptr_t>(scales) & 7) == 0 && ld_scales % 4 == 0;
+    p.vec_z = (reinterpret_cast<uintptr_t>(zeros) & 3) == 0 && ld_zeros % 4 == 0;
     // the longest slice that still gives every SM two CTAs
     const uint64_t row_blocks = (uint64_t(rows) + Q4_ROWS - 1) / Q4_ROWS;
     for (p.slice = 2048; p.slice > 512; p.slice /= 2) {
         const uint64_t n = (uint64_t(cols) + p.slice - 1) / p.slice;
         if (row_blocks * (n < Q4_MAX_RANKS ? n : Q4_MAX_RANKS) >= 296 && q4_smem_bytes(p.slice, group, n_vec > 8 ? 2 : 1, n_vec, zeros != nullptr) <= 112 * 1024) break;
     }
+    if (const char* e = getenv("DECXB200_Q4_SLICE")) p.slice = uint32_t(atoi(e));
     p.n_slices = (cols + p.slice - 1) / p.slice;
     p.ranks = p.n_slices < Q4_MAX_RANKS ? p.n_slices : Q4_MAX_RANKS;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -29,6 +29,7 @@ struct GemmQ8Params {
     void* D;
     uint64_t ldc, ldd;
     float alpha, beta;
+    int vec_d;                 // thin kernel: four neighbouring elements of D may be written at once
     int d_tma;                 // pair kernel: D through a staging tile and TMA stores (tmD); else per-thread stores
     int c_tma;                 // pair kernel, needs d_tma: C through TMA loads into the same staging tile (tmC)
     uint32_t tiles_m, tiles_n;
@@ -81,11 +82,66 @@ struct ThinCfg {
     static constexpr uint32_t STAGE = Q8_TILE + BN * Q8_KB;
     static constexpr int STAGES = (108 * 1024) / STAGE;               // two CTAs per SM
     static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + 1024 /*alignment slack*/ + 256 /*barriers*/;
+    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + 1024 /*alignment slack*/ + 256 /*barriers*/ + BN * 4 /*scales of A*/;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 128, BN);
     static_assert(STAGES * STAGE >= 128 * BN * 4, "the partial tile is exchanged in the ring");
     static_assert(16 * STAGES + 16 <= 256, "barrier area");
 };
+
+// four neighbouring columns of one row of D
+template <typename T>
+__device__ __forceinline__ void q8_put4(const GemmQ8Params& p, uint32_t m, uint32_t n, float (&d)[4]) {
+    T* at = static_cast<T*>(p.D) + uint64_t(m) * p.ldd + n;
+    if (p.C != nullptr) {
+        const T* c = static_cast<const T*>(p.C) + uint64_t(m) * p.ldc + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) d[i] = fmaf(p.beta, q8_to_f32(c[i]), d[i]);
+    }
+    if (p.vec_d && n + 4 <= p.N) {
+        if constexpr (sizeof(T) == 2) {
+            uint2 o;
+            q8_put(reinterpret_cast<T*>(&o) + 0, d[0]);
+            q8_put(reinterpret_cast<T*>(&o) + 1, d[1]);
+            q8_put(reinterpret_cast<T*>(&o) + 2, d[2]);
+            q8_put(reinterpret_cast<T*>(&o) + 3, d[3]);
+            *reinterpret_cast<uint2*>(at) = o;
+        } else {
+            *reinterpret_cast<float4*>(at) = make_float4(d[0], d[1], d[2], d[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) q8_put(at + i, d[i]);
+    }
+}
+
+// Adds the cluster's partial tiles ([token][128] floats at `partial` in every CTA) in rank order: this CTA's share.
+// All ranks' values of a unit are requested before the first is used: a remote access takes a few hundred cycles.
+template <int RANKS, typename T>
+__device__ __forceinline__ void q8_join(const GemmQ8Params& p, float* partial, const float* sa, uint32_t rank, uint32_t tm0,
+                                        uint32_t tn0, uint32_t tokens) {
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const float4* from[RANKS];
+#pragma unroll
+    for (int c = 0; c < RANKS; ++c) from[c] = reinterpret_cast<const float4*>(cluster.map_shared_rank(partial, c));
+    for (uint32_t i = rank * blockDim.x + threadIdx.x; i < tokens * 32; i += RANKS * blockDim.x) {
+        const uint32_t j = i >> 5, n = tn0 + (i & 31u) * 4;
+        if (n >= p.N) continue;
+        float4 v[RANKS];
+#pragma unroll
+        for (int c = 0; c < RANKS; ++c) v[c] = from[c][i];
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < RANKS; ++c) {
+            d[0] += v[c].x; d[1] += v[c].y; d[2] += v[c].z; d[3] += v[c].w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] *= sa[j] * (n + e < p.N ? p.alpha * __ldg(p.sb + n + e) : 0.f);
+        q8_put4<T>(p, tm0 + j, n, d);
+    }
+}
 
 template <int BN, typename T>
 __global__ void __launch_bounds__(192)
@@ -95,7 +151,9 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     extern __shared__ uint8_t q8_smem[];
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
     const uint32_t full = base + STAGES * Cfg::STAGE, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, slot = accf + 8;
-    float* partial = reinterpret_cast<float*>(q8_smem + (base - smem_u32(q8_smem)));       // [token][128], reuses the ring
+    uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
+    float* partial = reinterpret_cast<float*>(smem);                                       // [token][128], reuses the ring
+    float* sa = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE + 256);                // the tile's scales of A
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x % p.ranks, tile = blockIdx.x / p.ranks;
@@ -105,6 +163,8 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint64_t limit = p.wait_limit_ns;
 
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
@@ -116,10 +176,14 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_alloc<1>(slot, Cfg::TMEM_COLS);
         tmem_relinquish<1>();
     }
+    if (warp >= 2 && threadIdx.x - 64 < BN) {
+        const uint32_t m = tm * BN + threadIdx.x - 64;
+        sa[threadIdx.x - 64] = m < p.M ? p.sa[m] : 0.f;
+    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(q8_smem + (slot - smem_u32(q8_smem)));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
 
     bool ok = true;
     if (warp == 0) {
@@ -170,42 +234,41 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
     } else {
         const uint32_t quarter = warp & 3u;
+        const uint32_t n = tn * 128 + quarter * 32 + lane;
+        const float sbn = n < p.N ? p.alpha * __ldg(p.sb + n) : 0.f;
         if (!mbar_wait_bounded(accf, 0, limit)) {
             if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
             ok = false;
         }
         tc_fence_after_sync();
-        const uint32_t n = tn * 128 + quarter * 32 + lane;
         const uint32_t taddr = tmem + ((quarter * 32u) << 16);
         constexpr int CH = BN < 32 ? BN : 32;
-        if (p.ranks == 1) {
-            const float sbn = n < p.N ? p.alpha * p.sb[n] : 0.f;
 #pragma unroll 1
-            for (uint32_t c = 0; c < BN && ok; c += CH) {
-                if (tm * BN + c >= p.M) break;
-                uint32_t v[32];
-                tmem_ld_32x32(taddr + c, v);
-                tmem_ld_wait();
-                if (n < p.N) {
+        for (uint32_t c = 0; c < BN && ok; c += CH) {
+            const uint32_t m0 = tm * BN + c;
+            if (m0 >= p.M) break;
+            uint32_t v[32];
+            tmem_ld_32x32(taddr + c, v);
+            tmem_ld_wait();
+            if (p.ranks == 1) {
+                // lane = column: a warp writes 32 neighbouring elements of one row of D at a time
+                float d[CH];
 #pragma unroll
-                    for (int j = 0; j < CH; ++j) {
-                        const uint32_t m = tm * BN + c + j;
-                        if (m < p.M) {
-                            float d = __uint_as_float(v[j]) * (p.sa[m] * sbn);
-                            if (p.C != nullptr) d = fmaf(p.beta, q8_to_f32(static_cast<const T*>(p.C)[uint64_t(m) * p.ldc + n]), d);
-                            q8_put(static_cast<T*>(p.D) + uint64_t(m) * p.ldd + n, d);
-                        }
+                for (int j = 0; j < CH; ++j) d[j] = __uint_as_float(v[j]) * (sa[c + j] * sbn);
+                if (n < p.N) {
+                    if (p.C != nullptr) {
+                        const T* cp = static_cast<const T*>(p.C) + uint64_t(m0) * p.ldc + n;
+#pragma unroll
+                        for (int j = 0; j < CH; ++j)
+                            if (m0 + j < p.M) d[j] = fmaf(p.beta, q8_to_f32(cp[uint64_t(j) * p.ldc]), d[j]);
                     }
+                    T* dp = static_cast<T*>(p.D) + uint64_t(m0) * p.ldd + n;
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (m0 + j < p.M) q8_put(dp + uint64_t(j) * p.ldd, d[j]);
                 }
-            }
-        } else if (ok) {
-            // the ring is free: the MMAs that read it have completed
-#pragma unroll 1
-            for (uint32_t c = 0; c < BN; c += CH) {
-                if (tm * BN + c >= p.M) break;
-                uint32_t v[32];
-                tmem_ld_32x32(taddr + c, v);
-                tmem_ld_wait();
+            } else {
+                // the ring is free: the MMAs that read it have completed
 #pragma unroll
                 for (int j = 0; j < CH; ++j) partial[(c + j) * 128 + quarter * 32 + lane] = __uint_as_float(v[j]);
             }
@@ -218,21 +281,12 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
     }
     if (p.ranks > 1) {
-        namespace cg = cooperative_groups;
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
+        cluster_sync_all();
         const uint32_t tokens = min(uint32_t(BN), p.M - tm * BN);
-        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < tokens * 128; i += p.ranks * blockDim.x) {
-            const uint32_t m = tm * BN + i / 128, n = tn * 128 + i % 128;
-            float s = 0.f;
-            for (uint32_t c = 0; c < p.ranks; ++c) s += *cluster.map_shared_rank(partial + i, c);
-            if (n < p.N) {
-                float d = s * (p.sa[m] * (p.alpha * p.sb[n]));
-                if (p.C != nullptr) d = fmaf(p.beta, q8_to_f32(static_cast<const T*>(p.C)[uint64_t(m) * p.ldc + n]), d);
-                q8_put(static_cast<T*>(p.D) + uint64_t(m) * p.ldd + n, d);
-            }
-        }
-        cluster.sync();                                               // nobody leaves while its partial tile is being read
+        if (p.ranks == 2) q8_join<2, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
+        else if (p.ranks == 4) q8_join<4, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
+        else q8_join<8, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
+        cluster_sync_all();                                           // nobody leaves while its partial tile is being read
     }
 }
 
@@ -240,10 +294,13 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 struct PairCfg {
     static constexpr uint32_t STAGE = 2 * Q8_TILE;                    // 128 rows of A, 128 rows of B
     static constexpr int STAGES = 6;
-    static constexpr uint32_t STAGING = 4 * 4096;                     // per epilogue warp: 32 rows x 128 bytes of D
-    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+    static constexpr int EPI_WARPS = 8;                               // four lane quarters x two column halves
+    static constexpr uint32_t STAGING = EPI_WARPS * 4096;             // per epilogue warp: 32 rows x 128 bytes of D
+    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/ + 1024 /*scales of B*/;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 256, 256);
-    static constexpr int THREADS = 192;
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+    static_assert(16 * STAGES + 32 + 8 * EPI_WARPS + 8 <= 256, "barrier area");
+    static_assert(SMEM_BYTES <= 227 * 1024, "one CTA's shared memory");
 };
 
 __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p, uint32_t& tm, uint32_t& tn) {
@@ -254,10 +311,10 @@ __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p
     tn = r / rows;
 }
 
-// 32 finished columns col0.. of `row`, scaled, (+ beta * C), to the staging row (16-byte units unit0.., swizzled) or to D
+// 32 finished columns col0.. of `row`, scaled by sa * sb[0..31], (+ beta * C), to the staging row (16-byte units unit0.., swizzled) or to D
 template <typename T>
 __device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t row, uint32_t col0, const uint32_t (&v)[32], float sa,
-                                               uint32_t stage_row, uint32_t unit0, bool c_staged) {
+                                               const float* sb, uint32_t stage_row, uint32_t unit0, bool c_staged) {
     constexpr int PER = 16 / sizeof(T);                               // elements per 16-byte unit
     const uint32_t ncols = min(32u, p.N - col0), sw = (stage_row >> 7) & 7u;
     const bool has_c = p.C != nullptr && row < p.M;
@@ -267,9 +324,12 @@ __device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t r
     for (int u = 0; u < 32 / PER; ++u) {
         float d[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t j = u * PER + i;
-            d[i] = j < ncols ? __uint_as_float(v[j]) * (sa * __ldg(p.sb + col0 + j)) : 0.f;
+        for (int i = 0; i < PER; i += 4) {
+            const float4 b = reinterpret_cast<const float4*>(sb)[(u * PER + i) / 4];
+            d[i] = __uint_as_float(v[u * PER + i]) * (sa * b.x);
+            d[i + 1] = __uint_as_float(v[u * PER + i + 1]) * (sa * b.y);
+            d[i + 2] = __uint_as_float(v[u * PER + i + 2]) * (sa * b.z);
+            d[i + 3] = __uint_as_float(v[u * PER + i + 3]) * (sa * b.w);
         }
         if (has_c) {
             if (c_staged) {
@@ -306,7 +366,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
     const uint32_t staging = base + STAGES * PairCfg::STAGE;
     const uint32_t full = staging + PairCfg::STAGING, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, acce = accf + 16;
-    const uint32_t cbar0 = acce + 16, slot = cbar0 + 32;
+    const uint32_t cbar0 = acce + 16, slot = cbar0 + 8 * PairCfg::EPI_WARPS;
+    uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
+    float* const sb_tile = reinterpret_cast<float*>(smem + (full + 256 - base));       // the tile's 256 scales of B
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = cluster_ctarank();
@@ -322,9 +384,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(accf + 8 * a, 1);
-            mbar_init(acce + 8 * a, 8);                               // four epilogue warps of either CTA
+            mbar_init(acce + 8 * a, 2 * PairCfg::EPI_WARPS);          // the epilogue warps of both CTAs
         }
-        for (int w = 0; w < 4; ++w) mbar_init(cbar0 + 8 * w, 1);
+        for (int w = 0; w < PairCfg::EPI_WARPS; ++w) mbar_init(cbar0 + 8 * w, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -334,7 +396,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tc_fence_before_sync();
     cluster_sync_all();
     tc_fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(q8_smem + (slot - smem_u32(q8_smem)));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -414,7 +476,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
     } else {
         // ------------------------------------------------------------------ epilogue
-        const uint32_t quarter = warp & 3u;
+        const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;  // TMEM lanes [32 quarter, +32), columns [128 half, +128)
         const uint32_t acce0 = map_to_cta(acce, 0);
         const uint32_t stage_warp = staging + (warp - 2u) * 4096u;
         const uint32_t stage_row = p.d_tma ? stage_warp + lane * 128u : 0u;
@@ -426,21 +488,27 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const uint32_t cbar = cbar0 + 8 * (warp - 2u);
         uint32_t cph = 0, it = 0;
         bool ok = true;
-        for (uint32_t t = worker; t < n_tiles && ok; t += workers, ++it) {
+        for (uint32_t t = worker; t < n_tiles; t += workers, ++it) {
             uint32_t tm, tn;
             q8_tile_coords(t, p, tm, tn);
             const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane;
             const float sa = row < p.M ? p.alpha * p.sa[row] : 0.f;
+            // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more
+            const uint32_t sb_col = tn * 256 + threadIdx.x - 64;
+            const float sb_mine = sb_col < p.N ? __ldg(p.sb + sb_col) : 0.f;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            sb_tile[threadIdx.x - 64] = sb_mine;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             const uint32_t a = it & 1u, aph = (it >> 1) & 1u;
-            if (!mbar_wait_bounded(accf + 8 * a, aph, limit)) {
+            if (ok && !mbar_wait_bounded(accf + 8 * a, aph, limit)) {
                 if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-                break;
+                ok = false;                                           // keeps to the barriers above, touches nothing more
             }
             tc_fence_after_sync();
-            const uint32_t taddr = tmem + a * 256 + ((quarter * 32u) << 16);
+            const uint32_t taddr = tmem + a * 256 + half * 128 + ((quarter * 32u) << 16);
 #pragma unroll 1
-            for (uint32_t c = 0; c < 8; ++c) {
-                const uint32_t col0 = tn * 256 + c * 32;
+            for (uint32_t c = 0; c < 4 && ok; ++c) {
+                const uint32_t col0 = tn * 256 + half * 128 + c * 32;
                 if (col0 >= p.N) break;
                 uint32_t v[32];
                 tmem_ld_32x32(taddr + c * 32, v);
@@ -465,7 +533,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                             }
                         }
                     }
-                    q8_store_chunk<T>(p, row, col0, v, sa, stage_row, sub * (8 / SUB), c_box);
+                    q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + (col0 - tn * 256), stage_row, sub * (8 / SUB), c_box);
                     if (sub == SUB - 1 || col0 + 32 >= p.N) {
                         fence_proxy_async_smem();
                         __syncwarp();
@@ -475,12 +543,12 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         }
                     }
                 } else if (row < p.M) {
-                    q8_store_chunk<T>(p, row, col0, v, sa, 0, 0, false);
+                    q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + (col0 - tn * 256), 0, 0, false);
                 }
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acce0 + 8 * a);
+            if (lane == 0 && ok) mbar_arrive_cluster(acce0 + 8 * a);
         }
         if (lane == 0 && p.d_tma) bulk_wait_all();
     }

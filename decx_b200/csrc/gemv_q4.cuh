@@ -10,15 +10,17 @@
 //   * The products run on the warp-level tensor path, m16n8k16 with fp32 accumulators: 16 rows times up to 8 vectors
 //     per instruction, for the price of one vector.  tcgen05 would need the unpacked weights in shared memory, which
 //     costs more than the arithmetic.
-// Exactness.  A nibble q is put into the mantissa of an fp16 number (1024 + q, or 1024 + 16 q for the upper one of a
-// byte), from which one fp16 subtraction or fused multiply-add leaves exactly q - z.  x is fp16 or e4m3, which fp16
-// holds exactly.  Sums over a group are fp32, multiplied by the fp32 form of the group's scale and added in fp32;
-// the only other rounding is the one to an fp16 result.
+// Exactness and cost.  A nibble q left in the low bits of an fp16 number IS the subnormal q * 2^-24 (16 q * 2^-24 for the
+// upper nibble of a byte), and the tensor path multiplies subnormals exactly: one mask per pair of weights is all the
+// unpacking there is.  Products of lower and of upper nibbles go to accumulators of their own, and the zero point
+// leaves the sum: sum (q - z) x = sum q x - z sum x, with the group sums of x computed once per CTA.  x is fp16 or e4m3,
+// which fp16 holds exactly.  All sums are fp32; the group's scale multiplies in fp32; the only other rounding is the
+// one to an fp16 result.
 //
-// Order of K inside an instruction.  The lane that the instruction gives columns 2t, 2t+1, 2t+8, 2t+9 holds one 32-bit
-// word, weights 8t .. 8t+7 of a 32-weight step, and the unpacking yields pairs (0,4), (1,5), (2,6), (3,7).  Since a sum
-// does not care, x is staged in shared memory with each group of eight in that order and one 16-byte load of it
-// feeds both instructions of the step.
+// Order of K.  A sum does not care, so each lane takes whole words of a row: of a group of 32 / 64 / 128 weights the lane
+// that the instruction gives columns 2t, 2t+1, 2t+8, 2t+9 holds words t*w .. t*w+w-1 (w = 1 / 2 / 4, one shared-memory
+// load), and x is staged in shared memory in the order that this and the masks produce (0 4 2 6 1 5 3 7 within eight),
+// so that one 16-byte load feeds both instructions of a word.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -40,6 +42,7 @@ struct GemvQ4Params {
     uint32_t slice;            // weights of a row per CTA and round: 512, 1024 or 2048
     uint32_t n_slices;
     uint32_t ranks;            // CTAs of a row block = cluster size, at most 8
+    int vec_s, vec_z;          // four neighbouring scales / zero points may be read at once
 };
 
 constexpr int Q4_ROWS = 64;          // rows per CTA
@@ -48,16 +51,22 @@ constexpr int Q4_THREADS = 256;      // 2 row halves x 4 parts of the slice
 __host__ __device__ constexpr uint32_t q4_w_pitch(uint32_t slice) { return slice / 2; }
 // fp16 row of x: 64 bytes more than the slice, so that the two rows a quarter-warp reads fall on different banks
 __host__ __device__ constexpr uint32_t q4_x_pitch(uint32_t slice) { return slice * 2 + 64; }
+// a row's scales (fp32, or fp32 pairs with the zero point), padded against bank conflicts
+__host__ __device__ constexpr uint32_t q4_s_pitch(uint32_t groups, bool zeros) { return zeros ? (groups + 2) * 8 : (groups + 4) * 4; }
 __host__ __device__ constexpr uint32_t q4_red_bytes(uint32_t n_tiles) { return 4u * Q4_ROWS * (8 * n_tiles + 1) * 4; }
 __host__ __device__ constexpr uint32_t q4_smem_bytes(uint32_t slice, uint32_t group, uint32_t n_tiles, uint32_t n_vec,
                                                      bool zeros) {
     const uint32_t w = Q4_ROWS * q4_w_pitch(slice);
     const uint32_t x = n_vec * q4_x_pitch(slice);
-    const uint32_t s = Q4_ROWS * (slice / group + 1) * (zeros ? 8 : 4);
+    const uint32_t s = Q4_ROWS * q4_s_pitch(slice / group, zeros);
+    const uint32_t sums = slice / group * 8 * n_tiles * 4;                    // group sums of x
     const uint32_t red = q4_red_bytes(n_tiles) + Q4_ROWS * 8 * n_tiles * 4;   // reuses the weights' and x's space
-    const uint32_t total = w + x + s;
+    const uint32_t total = w + x + s + sums;
     return total > red ? total : red;
 }
+// 16-byte unit u of row r lies at unit u ^ q4_swizzle(r): loads of 4, 8 and 16 bytes per lane, eight rows by four
+// lanes, then meet no bank twice (bit-reversed row number within eight)
+__host__ __device__ constexpr uint32_t q4_swizzle(uint32_t r) { return ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -75,18 +84,27 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the first of a chain: d = a * b
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// a word of eight nibbles -> q - z as half2 pairs (0,4) (1,5) (2,6) (3,7); zl = 1024 + z twice, zh = 64 + z twice
-__device__ __forceinline__ void q4_unpack(uint32_t w, __half2 zl, __half2 zh, uint32_t (&o)[4]) {
-    const __half2 sixteenth = __float2half2_rn(0.0625f);
-    const uint32_t magic = 0x64006400u;
-    const uint32_t w8 = w >> 8;
-    o[0] = h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | magic), zl));
-    o[1] = h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | magic), sixteenth, __hneg2(zh)));
-    o[2] = h2_bits(__hsub2(bits_h2((w8 & 0x000f000fu) | magic), zl));
-    o[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00f000f0u) | magic), sixteenth, __hneg2(zh)));
+// W words (1, 2 or 4) from shared memory
+template <int W>
+__device__ __forceinline__ void q4_words(uint32_t at, uint32_t (&w)[W]) {
+    if constexpr (W == 1) {
+        w[0] = ld_shared_u32(at);
+    } else if constexpr (W == 2) {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    } else {
+        const uint4 v = ld_shared_v4(at);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    }
 }
 
 template <typename OUT>
@@ -98,12 +116,14 @@ template <> __device__ __forceinline__ __half q4_out<__half>(float v) { return _
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
 __global__ void __launch_bounds__(Q4_THREADS)
 gemv_q4_kernel(const GemvQ4Params p) {
-    extern __shared__ __align__(16) uint8_t q4_smem[];
+    extern __shared__ __align__(128) uint8_t q4_smem[];      // the swizzle works on address bits 4 to 6
+    constexpr int WPL = GROUP / 32;                           // words a lane holds of a row's group
+    constexpr int GU = GROUP / 8;                             // 16-byte units of x in a group
+    constexpr int NV = 8 * NT;
     const uint32_t base = smem_u32(q4_smem);
     const uint32_t wp = q4_w_pitch(p.slice), xp = q4_x_pitch(p.slice);
-    const uint32_t x_off = Q4_ROWS * wp, s_off = x_off + p.n_vec * xp;
-    constexpr uint32_t S_BYTES = ZEROS ? 8 : 4;               // fp32 scale, and 1024 + z twice in fp16
-    const uint32_t gps = p.slice / GROUP, s_pitch = (gps + 1) * S_BYTES;
+    const uint32_t gps = p.slice / GROUP, gps_log = 31 - __clz(gps), s_pitch = q4_s_pitch(gps, ZEROS);
+    const uint32_t x_off = Q4_ROWS * wp, s_off = x_off + p.n_vec * xp, xs_off = s_off + Q4_ROWS * s_pitch;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t half = warp & 1, part = warp >> 1;         // rows [32 half, +32), quarter `part` of the slice
     const uint32_t ranks = p.ranks, rank = blockIdx.x % ranks;
@@ -121,148 +141,176 @@ gemv_q4_kernel(const GemvQ4Params p) {
     for (uint32_t sl = rank; sl < p.n_slices; sl += ranks) {
         const uint32_t k0 = sl * p.slice;
         const uint32_t kn = min(p.slice, p.cols - k0);        // weights of a row in this slice
-        const uint32_t steps = (kn + 31) / 32;                // 32-weight steps
+        const uint32_t gn = (kn + GROUP - 1) / GROUP;         // its groups; the last one may be short
         if (sl != rank) __syncthreads();                      // the previous slice has been consumed
-        // ---- weights: 16-byte units, swizzled within groups of eight so that eight rows' words fall on all banks
-        const uint32_t units = steps;                         // 16 bytes = 32 weights
-        for (uint32_t i = threadIdx.x; i < Q4_ROWS * units; i += Q4_THREADS) {
-            const uint32_t r = i / units, u = i - r * units;
+        // ---- weights: warp w brings rows 8w .. 8w+7, a lane every 32nd 16-byte unit.  Bytes behind the row's end and
+        // rows behind the last one become zeros.
+        for (uint32_t u = lane; u < gn * (GROUP / 32); u += 32) {
             const uint32_t byte = k0 / 2 + u * 16;
-            const bool in = row0 + r < p.rows;
-            const uint32_t n = in ? min(16u, row_bytes - byte) : 0u;
-            const uint8_t* src = p.W + (in ? uint64_t(row0 + r) * p.ldw + byte : 0);
-            cp_async16(base + r * wp + ((u & ~7u) | ((u ^ r) & 7u)) * 16, src, n);
-        }
-        // ---- x as fp16, each group of eight in the order 0 4 1 5 2 6 3 7, zeros behind the last column
-        const uint32_t xunits = steps * 4;
-        for (uint32_t i = threadIdx.x; i < p.n_vec * xunits; i += Q4_THREADS) {
-            const uint32_t v = i / xunits, u = i - v * xunits, k = k0 + u * 8;
-            __half e[8];
-            if constexpr (X8) {
-                const uint8_t* src = static_cast<const uint8_t*>(p.x) + uint64_t(v) * p.ldx;
-                uint32_t b[2] = {0u, 0u};
-                if (k + 8 <= p.cols && ((reinterpret_cast<uintptr_t>(src + k)) & 7) == 0) {
-                    const uint2 d = *reinterpret_cast<const uint2*>(src + k);
-                    b[0] = d.x;
-                    b[1] = d.y;
-                } else {
+            const uint32_t n = byte < row_bytes ? min(16u, row_bytes - byte) : 0u;
+            const uint8_t* src = p.W + uint64_t(row0 + warp * 8) * p.ldw + byte;
+            const uint32_t dst = base + warp * 8 * wp + u * 16;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (k + j < p.cols) b[j >> 2] |= uint32_t(src[k + j]) << (8 * (j & 3));
+            for (uint32_t r = 0; r < 8; ++r) {
+                const bool in = n != 0 && row0 + warp * 8 + r < p.rows;
+                cp_async16((dst ^ (q4_swizzle(r) * 16)) + r * wp, in ? src : p.W, in ? n : 0u);
+                src += p.ldw;
+            }
+        }
+        // ---- x as fp16 in the order of the products, zeros behind the last column, and the sums of its groups
+        for (uint32_t v = 0; v < p.n_vec; ++v) {
+            for (uint32_t u = threadIdx.x; u < gps * GU; u += Q4_THREADS) {      // a multiple of 32: whole warps
+                const uint32_t k = k0 + u * 8;
+                uint32_t e[4];                                // pairs (0,1) (2,3) (4,5) (6,7)
+                if constexpr (X8) {
+                    const uint8_t* src = static_cast<const uint8_t*>(p.x) + uint64_t(v) * p.ldx + k;
+                    uint32_t b[2] = {0u, 0u};
+                    if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+                        const uint2 d = *reinterpret_cast<const uint2*>(src);
+                        b[0] = d.x;
+                        b[1] = d.y;
+                    } else if (k < p.cols) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (k + j < p.cols) b[j >> 2] |= uint32_t(src[j]) << (8 * (j & 3));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint16_t two = uint16_t(b[j >> 1] >> (16 * (j & 1)));
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(e[j]) : "h"(two));
+                    }
+                } else {
+                    const __half* src = static_cast<const __half*>(p.x) + uint64_t(v) * p.ldx + k;
+                    if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                        const uint4 d = *reinterpret_cast<const uint4*>(src);
+                        e[0] = d.x; e[1] = d.y; e[2] = d.z; e[3] = d.w;
+                    } else {
+                        __half h[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) h[j] = k + j < p.cols ? src[j] : __float2half(0.f);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) e[j] = h2_bits(__halves2half2(h[2 * j], h[2 * j + 1]));
+                    }
                 }
+                float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t h;
-                    const uint16_t two = uint16_t(b[j >> 1] >> (16 * (j & 1)));
-                    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-                    const __half2 hh = bits_h2(h);
-                    e[2 * j] = __low2half(hh);
-                    e[2 * j + 1] = __high2half(hh);
+                    const float2 f = __half22float2(bits_h2(e[j]));
+                    sum += f.x + f.y;
                 }
+#pragma unroll
+                for (int m = 1; m < GU; m *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+                const uint32_t gi = u / GU, w = u % GU;       // word w of the group belongs to lane w / WPL
+                if (w == 0) *reinterpret_cast<float*>(q4_smem + xs_off + (gi * NV + v) * 4) = sum * 0x1p-24f;
+                st_shared_v4(base + x_off + v * xp + (gi * GU + (w % WPL) * 4 + w / WPL) * 16,
+                             __byte_perm(e[0], e[2], 0x5410), __byte_perm(e[1], e[3], 0x5410),
+                             __byte_perm(e[0], e[2], 0x7632), __byte_perm(e[1], e[3], 0x7632));
+            }
+        }
+        // ---- scales (times 2^24) and zero points (negative), four neighbouring groups at a time
+        const uint32_t g0 = k0 / GROUP;
+        for (uint32_t i = threadIdx.x; i < Q4_ROWS * gps / 4; i += Q4_THREADS) {
+            const uint32_t r = i >> (gps_log - 2), gi = (i & (gps / 4 - 1)) * 4;
+            if (gi >= gn || row0 + r >= p.rows) continue;
+            const __half* sp = p.scales + uint64_t(row0 + r) * p.lds + g0 + gi;
+            float s[4], z[4];
+            if (p.vec_s && gi + 4 <= gn) {
+                const uint2 d = *reinterpret_cast<const uint2*>(sp);
+                const float2 a = __half22float2(bits_h2(d.x)), b = __half22float2(bits_h2(d.y));
+                s[0] = a.x; s[1] = a.y; s[2] = b.x; s[3] = b.y;
             } else {
-                const __half* src = static_cast<const __half*>(p.x) + uint64_t(v) * p.ldx;
-                if (k + 8 <= p.cols && ((reinterpret_cast<uintptr_t>(src + k)) & 15) == 0) {
-                    const uint4 d = *reinterpret_cast<const uint4*>(src + k);
-                    *reinterpret_cast<uint4*>(e) = d;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] = gi + j < gn ? __half2float(sp[j]) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] *= 0x1p24f;
+            const uint32_t at = base + s_off + r * s_pitch + gi * (ZEROS ? 8 : 4);
+            if constexpr (ZEROS) {
+                const uint8_t* zp = p.zeros + uint64_t(row0 + r) * p.ldz + g0 + gi;
+                if (p.vec_z && gi + 4 <= gn) {
+                    const uint32_t d = *reinterpret_cast<const uint32_t*>(zp);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) z[j] = -float((d >> (8 * j)) & 255u);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = k + j < p.cols ? src[k + j] : __float2half(0.f);
+                    for (int j = 0; j < 4; ++j) z[j] = gi + j < gn ? -float(zp[j]) : 0.f;
                 }
-            }
-            st_shared_v4(base + x_off + v * xp + u * 16, h2_bits(__halves2half2(e[0], e[4])),
-                         h2_bits(__halves2half2(e[1], e[5])), h2_bits(__halves2half2(e[2], e[6])),
-                         h2_bits(__halves2half2(e[3], e[7])));
-        }
-        // ---- scales (and zero points) of the slice
-        const uint32_t g0 = k0 / GROUP, gn = (kn + GROUP - 1) / GROUP;
-        for (uint32_t i = threadIdx.x; i < Q4_ROWS * gn; i += Q4_THREADS) {
-            const uint32_t r = i / gn, gi = i - r * gn;
-            const bool in = row0 + r < p.rows;
-            const float s = in ? __half2float(p.scales[uint64_t(row0 + r) * p.lds + g0 + gi]) : 0.f;
-            uint8_t* at = q4_smem + s_off + r * s_pitch + gi * S_BYTES;
-            if constexpr (ZEROS) {
-                const uint32_t z = in ? p.zeros[uint64_t(row0 + r) * p.ldz + g0 + gi] : 0u;
-                const __half2 zl = __half2half2(__uint2half_rn(1024u + z));
-                *reinterpret_cast<uint2*>(at) = make_uint2(__float_as_uint(s), h2_bits(zl));
+                st_shared_v4(at, __float_as_uint(s[0]), __float_as_uint(z[0]), __float_as_uint(s[1]), __float_as_uint(z[1]));
+                st_shared_v4(at + 16, __float_as_uint(s[2]), __float_as_uint(z[2]), __float_as_uint(s[3]), __float_as_uint(z[3]));
             } else {
-                *reinterpret_cast<float*>(at) = s;
+                st_shared_v4(at, __float_as_uint(s[0]), __float_as_uint(s[1]), __float_as_uint(s[2]), __float_as_uint(s[3]));
             }
         }
         cp_async_wait_all();
         __syncthreads();
 
-        // ---- multiply: this warp's 32 rows, its quarter of the slice in whole groups
-        const uint32_t per = ((gn + 3) / 4) * (GROUP / 32);   // steps of a quarter
-        const uint32_t st0 = part * per, st1 = min(steps, st0 + per);
-        const uint32_t wrow = base + (half * 32 + g) * wp;    // row g of the first tile; +8, +16, +24 rows follow
-        const uint32_t xrow = base + x_off;
-        for (uint32_t st = st0; st < st1; st += GROUP / 32) {
-            float gacc[2][NT][4];
+        // ---- multiply: this warp's 32 rows, its quarter of the slice's groups
+        const uint32_t per = (gn + 3) / 4, gi1 = min(gn, (part + 1) * per);
+        const uint32_t wrow = base + (half * 32 + g) * wp, sw = q4_swizzle(g) * 16;   // rows 8 apart share a swizzle
+        uint32_t xv[NT];                                      // lanes of vectors that do not exist read the last one;
+#pragma unroll                                                // their columns are never stored
+        for (int n = 0; n < NT; ++n) xv[n] = base + x_off + min(uint32_t(n * 8) + g, p.n_vec - 1) * xp + t * 16;
+#pragma unroll 1
+        for (uint32_t gi = part * per; gi < gi1; ++gi) {
+            uint32_t w[4][WPL];
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 4; ++m) q4_words<WPL>(wrow + m * 8 * wp + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), w[m]);
+            float lo[2][NT][4], hi[2][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int j = 0; j < WPL; ++j) {
+                uint4 xb[NT];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) gacc[m][n][i] = 0.f;
-            const uint32_t gi = st / (GROUP / 32);
-            float sc[4];
-            __half2 zl[4], zh[4];
+                for (int n = 0; n < NT; ++n) xb[n] = ld_shared_v4(xv[n] + (gi * GU + j * 4) * 16);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const uint32_t wa = w[2 * m][j], wb = w[2 * m + 1][j], wa8 = wa >> 8, wb8 = wb >> 8;
+                    constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if (j == 0) {
+                            mma_16816_first(lo[m][n], wa & L, wb & L, wa8 & L, wb8 & L, xb[n].x, xb[n].y);
+                            mma_16816_first(hi[m][n], wa & H, wb & H, wa8 & H, wb8 & H, xb[n].z, xb[n].w);
+                        } else {
+                            mma_16816(lo[m][n], wa & L, wb & L, wa8 & L, wb8 & L, xb[n].x, xb[n].y);
+                            mma_16816(hi[m][n], wa & H, wb & H, wa8 & H, wb8 & H, xb[n].z, xb[n].w);
+                        }
+                    }
+                }
+            }
+            float sc[4], nz[4];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const uint32_t at = base + s_off + (half * 32 + m * 8 + g) * s_pitch + gi * S_BYTES;
+                const uint32_t at = base + s_off + (half * 32 + m * 8 + g) * s_pitch + gi * (ZEROS ? 8 : 4);
                 if constexpr (ZEROS) {
-                    uint32_t a, b;
-                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(at));
-                    sc[m] = __uint_as_float(a);
-                    zl[m] = bits_h2(b);
-                    zh[m] = __hsub2(zl[m], __float2half2_rn(960.f));
+                    uint32_t v[2];
+                    q4_words<2>(at, v);
+                    sc[m] = __uint_as_float(v[0]);
+                    nz[m] = __uint_as_float(v[1]);
                 } else {
                     sc[m] = __uint_as_float(ld_shared_u32(at));
-                    zl[m] = __float2half2_rn(1032.f);
-                    zh[m] = __float2half2_rn(72.f);
+                    nz[m] = -8.f;
                 }
             }
 #pragma unroll
-            for (int j = 0; j < GROUP / 32; ++j) {
-                const uint32_t u = st + j;
-                if (GROUP > 32 && u >= st1) break;            // the last group of the row is short
-                uint4 xb[NT];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    // lanes of vectors that do not exist read the last one; their columns are never stored
-                    const uint32_t v = min(uint32_t(n * 8) + g, p.n_vec - 1);
-                    xb[n] = ld_shared_v4(xrow + v * xp + (u * 4 + t) * 16);
-                }
-                uint32_t a[4][4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    // rows m * 8 + g: all have the same row & 7 = g, hence the same swizzle
-                    const uint32_t w = ld_shared_u32(wrow + m * 8 * wp + ((u & ~7u) | ((u ^ g) & 7u)) * 16 + t * 4);
-                    q4_unpack(w, zl[m], zh[m], a[m]);
-                }
+            for (int n = 0; n < NT; ++n) {
+                uint32_t v[2];
+                q4_words<2>(base + xs_off + (gi * NV + n * 8 + 2 * t) * 4, v);
+                const float xs[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_16816(gacc[m][n], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], xb[n].x, xb[n].y);
-                        mma_16816(gacc[m][n], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], xb[n].z, xb[n].w);
+                    for (int i = 0; i < 4; ++i) {             // i >> 1: row g or g + 8; i & 1: vector 2t or 2t + 1
+                        float d = fmaf(hi[m][n][i], 0.0625f, lo[m][n][i]);
+                        d = fmaf(nz[2 * m + (i >> 1)], xs[i & 1], d);
+                        acc[m][n][i] = fmaf(sc[2 * m + (i >> 1)], d, acc[m][n][i]);
                     }
             }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    acc[m][n][0] = fmaf(sc[2 * m], gacc[m][n][0], acc[m][n][0]);
-                    acc[m][n][1] = fmaf(sc[2 * m], gacc[m][n][1], acc[m][n][1]);
-                    acc[m][n][2] = fmaf(sc[2 * m + 1], gacc[m][n][2], acc[m][n][2]);
-                    acc[m][n][3] = fmaf(sc[2 * m + 1], gacc[m][n][3], acc[m][n][3]);
-                }
         }
     }
 
     // ---- join: the four quarters through shared memory, then the slices through distributed shared memory
     __syncthreads();
-    constexpr int NV = 8 * NT, RP = NV + 1;
+    constexpr int RP = NV + 1;
     float* red = reinterpret_cast<float*>(q4_smem);                       // [part][row][RP]
     float* sums = red + 4 * Q4_ROWS * RP;                                 // [vector][row]
 #pragma unroll
@@ -272,32 +320,38 @@ gemv_q4_kernel(const GemvQ4Params p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t r = half * 32 + m * 16 + g + (i >> 1) * 8, v = n * 8 + 2 * t + (i & 1);
-                red[(part * Q4_ROWS + r) * RP + v] = acc[m][n][i];
+                if (v < p.n_vec) red[(part * Q4_ROWS + r) * RP + v] = acc[m][n][i];
             }
     __syncthreads();
+    auto store = [&](uint32_t v, uint32_t r, float s) {
+        if (row0 + r < p.rows) {
+            if (p.xs != nullptr) s *= __ldg(p.xs + v);
+            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row0 + r] = q4_out<OUT>(s);
+        }
+    };
     for (uint32_t i = threadIdx.x; i < Q4_ROWS * p.n_vec; i += Q4_THREADS) {
         const uint32_t v = i / Q4_ROWS, r = i % Q4_ROWS;
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) s += red[(q * Q4_ROWS + r) * RP + v];
-        sums[i] = s;
+        if (ranks > 1) sums[i] = s;
+        else store(v, r, s);
     }
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    if (ranks > 1) cluster.sync(); else __syncthreads();
-    for (uint32_t i = rank * Q4_THREADS + threadIdx.x; i < Q4_ROWS * p.n_vec; i += ranks * Q4_THREADS) {
-        const uint32_t v = i / Q4_ROWS, r = i % Q4_ROWS;
-        float s = 0.f;
-        if (ranks > 1)
-            for (uint32_t c = 0; c < ranks; ++c) s += *cluster.map_shared_rank(sums + i, c);
-        else
-            s = sums[i];
-        if (row0 + r < p.rows) {
-            if (p.xs != nullptr) s *= p.xs[v];
-            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row0 + r] = q4_out<OUT>(s);
+    if (ranks > 1) {
+        namespace cg = cooperative_groups;
+        const cg::cluster_group cluster = cg::this_cluster();
+        cluster_sync_all();
+        for (uint32_t i = rank * Q4_THREADS + threadIdx.x; i < Q4_ROWS * p.n_vec; i += ranks * Q4_THREADS) {
+            float d[8];                                                   // requested together, added in slice order
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) d[c] = c < ranks ? *cluster.map_shared_rank(sums + i, c) : 0.f;
+            float s = 0.f;
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) s += d[c];
+            store(i / Q4_ROWS, i % Q4_ROWS, s);
         }
+        cluster_sync_all();                                               // nobody leaves while its sums are being read
     }
-    if (ranks > 1) cluster.sync();                            // nobody leaves while its sums are being read
 }
 
 }  // namespace dxb

@@ -15,6 +15,8 @@
 #include <cuda_fp16.h>
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace dxb {
 
 struct RowQ8Params {
@@ -27,6 +29,7 @@ struct RowQ8Params {
     uint64_t ldx, ldr, lds, ldq;
     uint32_t rows, cols;
     float eps;
+    uint32_t depth;            // ring kernel: rows in the ring, 2 to 4
 };
 
 constexpr float E4M3_MAX = 448.f;
@@ -209,6 +212,285 @@ row_q8_kernel(const RowQ8Params p) {
                     const uint32_t k = col + (VEC ? i : i * tpr);
                     if (k < p.cols) q[k] = uint8_t(e4m3x2(v[c][i], 0.f));
                 }
+            }
+        }
+    }
+}
+
+// ---- ring kernel -------------------------------------------------------------------------------------------
+// Many rows: what limits row_q8_kernel is that a CTA's loads, reduction and stores follow one another (fp16
+// cast of 4096 x 16384: 72 us against 31 us of traffic).  Here the CTAs stay, and every thread asks for its own pieces
+// of the rows to come with asynchronous copies into its own slots of a ring in shared memory.  Nobody else reads a slot,
+// so the ring needs no barrier; the only one per row is the reduction's.
+//
+// SHIFT: rows of x, r and sum that start anywhere (an odd row length).  A thread then copies the aligned 16-byte units that
+// its 8 elements touch and shifts them into place; on the way out the lanes of a warp pass each other what an aligned
+// unit of the other side needs.
+
+__device__ __forceinline__ void q8_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// SHIFT: neighbouring threads ask for overlapping units, so these go through L1
+__device__ __forceinline__ void q8_async16_l1(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void q8_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all but the newest `ahead` groups of this thread have landed
+__device__ __forceinline__ void q8_async_wait(uint32_t ahead) {
+    if (ahead == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
+
+// N words of `s` from byte `o` (below 16; whole words only when WORDS) on
+template <bool WORDS, int WS, int N, int S>
+__device__ __forceinline__ void q8_pick_at(const uint32_t (&s)[S], uint32_t o, uint32_t (&out)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (WORDS) out[i] = s[WS + i];
+        else out[i] = __funnelshift_r(s[WS + i], s[WS + i + 1 < S ? WS + i + 1 : S - 1], (o & 2) * 8);
+    }
+}
+template <bool WORDS, int N, int S>
+__device__ __forceinline__ void q8_pick(const uint32_t (&s)[S], uint32_t o, uint32_t (&out)[N]) {
+    switch (o >> 2) {                                     // the same for a whole row
+        case 0: q8_pick_at<WORDS, 0, N, S>(s, o, out); break;
+        case 1: q8_pick_at<WORDS, 1, N, S>(s, o, out); break;
+        case 2: q8_pick_at<WORDS, 2, N, S>(s, o, out); break;
+        default: q8_pick_at<WORDS, 3, N, S>(s, o, out); break;
+    }
+}
+
+__device__ __forceinline__ void q8_to_floats(const uint32_t (&w)[4], float (&f)[8], __half) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = a.x;
+        f[2 * i + 1] = a.y;
+    }
+}
+__device__ __forceinline__ void q8_to_floats(const uint32_t (&w)[8], float (&f)[8], float) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+}
+
+// 8 elements per lane, consecutive over the warp, to a row that starts anywhere; every lane has all 8
+template <typename T>
+__device__ __forceinline__ void q8_store8_shift(T* at, const float (&f)[8], uint32_t lane) {
+    constexpr int W = 8 * sizeof(T) / 4;                  // words of a lane
+    uint32_t s[W + 4];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            s[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = __float_as_uint(f[i]);
+    }
+    const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+    if (o == 0) {
+#pragma unroll
+        for (int u = 0; u < W / 4; ++u)
+            reinterpret_cast<uint4*>(at)[u] = make_uint4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[W + i] = __shfl_down_sync(0xffffffffu, s[i], 1);
+    const uint32_t d = 16 - o, head = d / sizeof(T);      // the first aligned unit starts this many elements in
+    uint32_t out[W];
+    q8_pick<sizeof(T) == 4, W, W + 4>(s, d, out);
+    uint4* unit = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + d);
+#pragma unroll
+    for (int u = 0; u < W / 4; ++u)
+        if (lane < 31 || u + 1 < W / 4) unit[u] = make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
+    // what lies before the warp's first and behind its last whole unit
+    const uint32_t tail = head + 8 * (W / 4 - 1) / (W / 4);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if ((lane == 0 && i < head) || (lane == 31 && i >= tail)) q8_store(at + i, f[i]);
+}
+
+template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
+__global__ void __launch_bounds__(WARP ? 256 : 1024)
+row_q8_ring_kernel(const RowQ8Params p) {
+    extern __shared__ __align__(128) uint8_t q8_ring[];
+    __shared__ float red_ss[2][32];
+    __shared__ uint32_t red_top[2][32];
+    constexpr int U = 8 * sizeof(T) / 16, UL = U + (SHIFT ? 1 : 0);   // 16-byte units of 8 elements, and loaded
+    constexpr int UT = UL * (RES ? 2 : 1);
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t tpr = WARP ? 32u : blockDim.x, tid = WARP ? lane : threadIdx.x;
+    const uint32_t step = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+    const uint32_t first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const uint32_t unit_step = blockDim.x * 16;                       // a thread's units lie this far apart
+    const uint32_t mine = smem_u32(q8_ring) + threadIdx.x * 16;
+    const T* const w = static_cast<const T*>(p.w);
+
+    // ask for this thread's pieces of a row
+    auto request = [&](uint32_t slot, const T* mat, uint64_t ld, uint64_t row, int u0) {
+        const T* const rp = mat + row * ld;
+        const uint8_t* const end = reinterpret_cast<const uint8_t*>(rp + p.cols);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const uint32_t col = (c * tpr + tid) * 8;
+            if (col >= p.cols) continue;
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(rp + col);
+            const uint32_t dst = mine + ((slot * NCH + c) * UT + u0) * unit_step;
+            if constexpr (SHIFT) {
+                const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+                at -= o;
+                if (at < reinterpret_cast<const uint8_t*>(mat)) {     // the matrix itself starts inside this unit
+                    T* const own = reinterpret_cast<T*>(q8_ring + (dst - smem_u32(q8_ring)));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t b = o + i * sizeof(T);         // byte within the units, which lie unit_step apart
+                        own[(b / 16 * unit_step + b % 16) / sizeof(T)] = col + i < p.cols ? rp[col + i] : T(0.f);
+                    }
+                    continue;
+                }
+                if (o == 0) {                                         // nothing of the last unit is needed
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int64_t left = end - (at + u * 16);
+                        q8_async16_l1(dst + u * unit_step, left > 0 ? at + u * 16 : at, left >= 16 ? 16u : (left > 0 ? uint32_t(left) : 0u));
+                    }
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UL; ++u) {
+                const int64_t left = end - (at + u * 16);
+                const uint32_t n = left >= 16 ? 16u : (left > 0 ? uint32_t(left) : 0u);
+                if constexpr (SHIFT) q8_async16_l1(dst + u * unit_step, n ? at + u * 16 : at, n);
+                else q8_async16(dst + u * unit_step, n ? at + u * 16 : at, n);
+            }
+        }
+    };
+    auto request_row = [&](uint32_t slot, uint64_t row) {
+        if (row < p.rows) {
+            request(slot, static_cast<const T*>(p.x), p.ldx, row, 0);
+            if constexpr (RES) request(slot, static_cast<const T*>(p.r), p.ldr, row, UL);
+        }
+        q8_async_commit();
+    };
+    auto take = [&](uint32_t slot, int c, const T* mat, uint64_t ld, uint64_t row, int u0, float (&f)[8]) {
+        const uint32_t src = mine + ((slot * NCH + c) * UT + u0) * unit_step;
+        uint32_t s[4 * UL], o4[4 * U];
+#pragma unroll
+        for (int u = 0; u < UL; ++u) {
+            const uint4 v = ld_shared_v4(src + u * unit_step);
+            s[4 * u] = v.x; s[4 * u + 1] = v.y; s[4 * u + 2] = v.z; s[4 * u + 3] = v.w;
+        }
+        if constexpr (SHIFT) {
+            q8_pick<sizeof(T) == 4, 4 * U, 4 * UL>(s, uint32_t(reinterpret_cast<uintptr_t>(mat + row * ld)) & 15u, o4);
+            q8_to_floats(o4, f, T());
+        } else {
+            q8_to_floats(s, f, T());
+        }
+    };
+
+    uint64_t ahead = first;                                           // the next row to ask for
+    uint32_t put = 0, get = 0, odd = 0;
+    for (uint32_t d = 0; d + 1 < p.depth; ++d, ahead += step) {
+        request_row(put, ahead);
+        if (++put == p.depth) put = 0;
+    }
+    for (uint64_t row = first; row < p.rows; row += step, odd ^= 1u) {
+        request_row(put, ahead);
+        ahead += step;
+        if (++put == p.depth) put = 0;
+        q8_async_wait(p.depth - 1);
+        T* const sum = RES && p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.lds : nullptr;
+        uint8_t* const q = p.q + row * p.ldq;
+        float v[NCH][8];
+        float ss = 0.f, big = 0.f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const uint32_t col = (c * tpr + tid) * 8;
+            const bool any = col < p.cols, all = col + 8 <= p.cols;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+            if (any) take(get, c, static_cast<const T*>(p.x), p.ldx, row, 0, v[c]);
+            if constexpr (RES) {
+                float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (any) take(get, c, static_cast<const T*>(p.r), p.ldr, row, UL, a);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] += a[i];
+                if (sum != nullptr) {
+                    if (SHIFT && (c * tpr + (tid | 31u)) * 8 + 8 <= p.cols) {          // the whole warp has whole pieces
+                        q8_store8_shift(sum + col, v[c], lane);
+                    } else if (!SHIFT && all) {
+                        q8_store8(sum + col, v[c]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (col + i < p.cols) q8_store(sum + col + i, v[c][i]);
+                    }
+                }
+            }
+            if constexpr (NORM) {
+                float a[8];
+                if (all) {
+                    q8_load8(w + col, a);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a[i] = col + i < p.cols ? q8_load(w + col + i) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss = fmaf(v[c][i], v[c][i], ss);
+                    v[c][i] *= a[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(big) : "f"(fabsf(v[c][i])));
+        }
+        if (++get == p.depth) get = 0;
+        // ---- the row's sum of squares and largest magnitude (two sets of slots: one barrier a row)
+        uint32_t top = __float_as_uint(big);
+        if constexpr (NORM) {
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if constexpr (!WARP) {
+            const uint32_t wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
+            if (lane == 0) {
+                red_ss[odd][wid] = ss;
+                red_top[odd][wid] = top;
+            }
+            __syncthreads();
+            top = lane < warps ? red_top[odd][lane] : 0u;
+            if constexpr (NORM) {
+                ss = lane < warps ? red_ss[odd][lane] : 0.f;
+#pragma unroll
+                for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+        }
+        float scale, pre, mul;
+        q8_factors<NORM>(p, ss, top, scale, pre, mul);
+        if (tid == 0) p.scales[row] = scale;
+        if (pre != 1.f) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] *= pre;
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const uint32_t col = (c * tpr + tid) * 8;
+            uint2 o;
+            o.x = e4m3x2(v[c][0] * mul, v[c][1] * mul) | (e4m3x2(v[c][2] * mul, v[c][3] * mul) << 16);
+            o.y = e4m3x2(v[c][4] * mul, v[c][5] * mul) | (e4m3x2(v[c][6] * mul, v[c][7] * mul) << 16);
+            if (col + 8 <= p.cols) {
+                *reinterpret_cast<uint2*>(q + col) = o;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (col + i < p.cols) q[col + i] = uint8_t((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
             }
         }
     }

@@ -191,7 +191,7 @@ def test_quantised_layer(G, dev, tokens):
         torch.cuda.synchronize()
         w4 = (q4.double() - 8) * s4.double().repeat_interleave(group, 1)
         xq = q.float().double() * s.double()[:, None]
-        tol = (H / 16 + 32) * 2.0 ** -23 * (xq.abs() @ w4.abs().t())
+        tol = (H / 16 + 32) * 2.0 ** -23 * (xq.abs() @ ((q4.double() + 8) * s4.double().repeat_interleave(group, 1)).t())
         assert torch.all((y4.double() - xq @ w4.t()).abs() <= tol)
 
 

@@ -42,12 +42,13 @@ def _case(dev, rows, cols, group, n, zeros, x8, seed, pad=0):
 
 
 def _exact(q, s, z, v, xs, group):
-    """The result, and the sum of the magnitudes of its terms."""
+    """The result, and the sum of the magnitudes of its terms: q x and z x are summed apart."""
     cols = q.shape[1]
     at = torch.arange(cols, device=q.device) // group
-    w = (q.double() - (z.double()[:, at] if z is not None else 8.0)) * s.double()[:, at]
+    zero = z.double()[:, at] if z is not None else 8.0
+    w = (q.double() - zero) * s.double()[:, at]
     x = v.float().double() * (xs.double()[:, None] if xs is not None else 1.0)
-    return x @ w.t(), x.abs() @ w.abs().t()
+    return x @ w.t(), x.abs() @ ((q.double() + zero) * s.double()[:, at]).t()
 
 
 def _check(y, ref, mag, cols):
