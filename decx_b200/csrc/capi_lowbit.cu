@@ -42,8 +42,8 @@ int sm_count() {
 
 template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
 int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
-    constexpr uint32_t U = 8 * sizeof(T) / 16 + (SHIFT ? 1 : 0);
-    const uint32_t row = threads * NCH * U * (RES ? 2 : 1) * 16;      // one slot of the ring
+    constexpr uint32_t UNITS = NCH * 8 * sizeof(T) / 16 * (RES ? 2 : 1);
+    const uint32_t row = threads / 32 * (SHIFT ? 33 : 32) * 16 * UNITS;      // one slot of the ring
     auto kern = row_q8_ring_kernel<T, NORM, RES, WARP, SHIFT, NCH>;
     static std::atomic<uint64_t> done{0};
     static std::atomic<int> regs{0};
@@ -110,7 +110,7 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
                         (p.sum == nullptr || (aligned16(p.sum) && (p.lds * e) % 16 == 0));
     const bool out8 = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 && aligned16(p.w);
     // two slots of the ring have to fit: the limit is 1024 threads times two pieces of 8, or shared memory
-    const uint64_t slot = uint64_t(p.cols + 511) / 512 * 512 * (e + (rows16 ? 0 : 2)) * (p.r != nullptr ? 2 : 1);
+    const uint64_t slot = uint64_t(p.cols + 511) / 512 * (rows16 ? 512 : 528) * e * (p.r != nullptr ? 2 : 1);
     const bool ring = out8 && p.cols <= 16384 && 2 * slot <= 200 * 1024 && (p.rows > 296 || !rows16);
     if (!ring) return rows16 && out8 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
     if constexpr (NORM) {
@@ -120,21 +120,26 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     return rows16 ? launch_row_q8_shape<T, NORM, false, false>(s, p) : launch_row_q8_shape<T, NORM, false, true>(s, p);
 }
 
-template <typename K, typename... Args>
-int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t s, const Args&... args) {
-    cudaLaunchConfig_t cfg;
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[1], unsigned blocks, unsigned threads, unsigned smem,
+                    unsigned cluster, cudaStream_t s) {
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+}
+
+template <typename K, typename... Args>
+int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    cluster_config(cfg, attr, blocks, threads, smem, cluster, s);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
     if (e != cudaSuccess) return int(e);
     dxb_host::count_launch();
@@ -144,14 +149,46 @@ int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, uns
 constexpr uint32_t Q4_MAX_VEC = 16, Q4_MAX_RANKS = 8;
 
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
-int launch_gemv_q4(cudaStream_t s, const GemvQ4Params& p) {
+int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
+    using Cfg = Q4Cfg<NT>;
     auto kern = gemv_q4_kernel<GROUP, NT, ZEROS, X8, OUT>;
     static std::atomic<uint64_t> done{0};
-    const int rc = allow_smem(kern, 227 * 1024, done);
+    int rc = allow_smem(kern, Cfg::smem(Cfg::WARPS), done);
     if (rc != 0) return rc;
-    const uint64_t blocks = (uint64_t(p.rows) + Q4_ROWS - 1) / Q4_ROWS * p.ranks;
-    if (blocks > 0x7fffffffull) return DECXB200_ETOOLARGE;
-    return launch_cluster(kern, unsigned(blocks), Q4_THREADS, q4_smem_bytes(p.slice, GROUP, NT, p.n_vec, ZEROS), p.ranks, s, p);
+    const uint32_t pieces = (p.cols + Cfg::KW - 1) / Cfg::KW;
+    p.ranks = (pieces + Cfg::WARPS - 1) / Cfg::WARPS;
+    if (p.ranks > Q4_MAX_RANKS) p.ranks = Q4_MAX_RANKS;
+    uint32_t warps = (pieces + p.ranks - 1) / p.ranks;
+    if (warps > uint32_t(Cfg::WARPS)) warps = Cfg::WARPS;
+    p.passes = (pieces + p.ranks * warps - 1) / (p.ranks * warps);
+    constexpr uint32_t GC = Cfg::KW / GROUP;
+    p.vec_s = reinterpret_cast<uintptr_t>(p.scales) % (2 * GC) == 0 && p.lds % GC == 0;
+    p.vec_z = reinterpret_cast<uintptr_t>(p.zeros) % GC == 0 && p.ldz % GC == 0;
+    // clusters the GPU holds at once: the grid, since they stay and take turns over the blocks of rows
+    static std::atomic<int> held[Q4_MAX_RANKS][Cfg::WARPS];
+    int clusters = held[p.ranks - 1][warps - 1].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr[1];
+        cluster_config(cfg, attr, p.ranks, 32 * warps, Cfg::smem(warps), p.ranks, s);
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+        if (e != cudaSuccess) return int(e);
+        if (clusters < 1) clusters = 1;
+        held[p.ranks - 1][warps - 1].store(clusters, std::memory_order_relaxed);
+    }
+    // the height of the blocks that is done in the fewest turns (the larger one of equals: fewer joins)
+    uint64_t best = ~0ull;
+    for (uint32_t tiles = Cfg::MAX_TILES; tiles >= 1; tiles /= 2) {
+        const uint64_t blocks = (uint64_t(p.rows) + 16 * tiles - 1) / (16 * tiles);
+        const uint64_t turns = (blocks + clusters - 1) / clusters * tiles;
+        if (turns < best) {
+            best = turns;
+            p.tiles = tiles;
+        }
+    }
+    const uint64_t blocks = (uint64_t(p.rows) + 16 * p.tiles - 1) / (16 * p.tiles);
+    const uint64_t n = blocks < uint64_t(clusters) ? blocks : uint64_t(clusters);
+    return launch_cluster(kern, unsigned(n * p.ranks), 32 * warps, Cfg::smem(warps), p.ranks, s, p);
 }
 
 template <int GROUP, int NT, bool ZEROS>
@@ -190,18 +227,16 @@ int launch_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
 
 template <typename T>
 int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
-    CUtensorMap ma, mb, md, mc;
+    CUtensorMap ma, mb, md;
     int rc;
     if ((rc = dxb_host::tensor_map_2d(&ma, 1, A, p.M, p.K, lda, Q8_KB, 128)) != 0) return rc;
     if ((rc = dxb_host::tensor_map_2d(&mb, 1, B, p.N, p.K, ldb, Q8_KB, 128)) != 0) return rc;
-    md = mc = ma;
+    md = ma;
     const uint64_t e = sizeof(T);
     if (aligned16(p.D) && (p.ldd * e) % 16 == 0 &&
         dxb_host::tensor_map_2d(&md, int(e), p.D, p.M, p.N, p.ldd, uint32_t(128 / e), 32) == 0)
         p.d_tma = 1;
-    if (p.d_tma && p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0 &&
-        dxb_host::tensor_map_2d(&mc, int(e), p.C, p.M, p.N, p.ldc, uint32_t(128 / e), 32) == 0)
-        p.c_tma = 1;
+    p.vec_c = p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0;
     auto kern = gemm_q8_pair_kernel<T>;
     static std::atomic<uint64_t> done{0};
     if ((rc = allow_smem(kern, PairCfg::SMEM_BYTES, done)) != 0) return rc;
@@ -213,7 +248,7 @@ int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
     uint64_t pairs = uint64_t(sm_count()) / 2;
     if (pairs > tiles) pairs = tiles;
     if (pairs == 0) pairs = 1;
-    return launch_cluster(kern, unsigned(2 * pairs), PairCfg::THREADS, PairCfg::SMEM_BYTES, 2, s, ma, mb, md, mc, p);
+    return launch_cluster(kern, unsigned(2 * pairs), PairCfg::THREADS, PairCfg::SMEM_BYTES, 2, s, ma, mb, md, p);
 }
 
 template <typename T>
@@ -287,17 +322,6 @@ int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint
     p.x = x; p.ldx = ldx; p.xs = x_scales;
     p.y = y; p.ldy = ldy;
     p.rows = rows; p.cols = cols; p.n_vec = n_vec;
-    p.vec_s = (reinterpret_cast<uintptr_t>(scales) & 7) == 0 && ld_scales % 4 == 0;
-    p.vec_z = (reinterpret_cast<uintptr_t>(zeros) & 3) == 0 && ld_zeros % 4 == 0;
-    // the longest slice that still gives every SM two CTAs
-    const uint64_t row_blocks = (uint64_t(rows) + Q4_ROWS - 1) / Q4_ROWS;
-    for (p.slice = 2048; p.slice > 512; p.slice /= 2) {
-        const uint64_t n = (uint64_t(cols) + p.slice - 1) / p.slice;
-        if (row_blocks * (n < Q4_MAX_RANKS ? n : Q4_MAX_RANKS) >= 296 && q4_smem_bytes(p.slice, group, n_vec > 8 ? 2 : 1, n_vec, zeros != nullptr) <= 112 * 1024) break;
-    }
-    if (const char* e = getenv("DECXB200_Q4_SLICE")) p.slice = uint32_t(atoi(e));
-    p.n_slices = (cols + p.slice - 1) / p.slice;
-    p.ranks = p.n_slices < Q4_MAX_RANKS ? p.n_slices : Q4_MAX_RANKS;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const bool x8 = x_dtype == DECXB200_E4M3, f32 = y_dtype == DECXB200_FP32;
     if (group == 32) return run_gemv_q4_group<32>(s, x8, f32, p);

@@ -31,7 +31,7 @@ struct GemmQ8Params {
     float alpha, beta;
     int vec_d;                 // thin kernel: four neighbouring elements of D may be written at once
     int d_tma;                 // pair kernel: D through a staging tile and TMA stores (tmD); else per-thread stores
-    int c_tma;                 // pair kernel, needs d_tma: C through TMA loads into the same staging tile (tmC)
+    int vec_c;                 // pair kernel: rows of C are 16-byte aligned
     uint32_t tiles_m, tiles_n;
     uint32_t group_m;          // pair kernel: height of the rasterisation groups, in tiles
     uint32_t ranks;            // thin kernel: CTAs that share a tile's K = cluster size
@@ -299,7 +299,7 @@ struct PairCfg {
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/ + 1024 /*scales of B*/;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 256, 256);
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static_assert(16 * STAGES + 32 + 8 * EPI_WARPS + 8 <= 256, "barrier area");
+    static_assert(16 * STAGES + 32 + 8 <= 256, "barrier area");
     static_assert(SMEM_BYTES <= 227 * 1024, "one CTA's shared memory");
 };
 
@@ -311,15 +311,29 @@ __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p
     tn = r / rows;
 }
 
-// 32 finished columns col0.. of `row`, scaled by sa * sb[0..31], (+ beta * C), to the staging row (16-byte units unit0.., swizzled) or to D
+// 32 columns col0.. of one row of C, if there are that many: a lane reads whole 128-byte lines (64 for fp16)
+template <typename T>
+__device__ __forceinline__ void q8_load_c(const GemmQ8Params& p, uint32_t row, uint32_t col0, uint4 (&c)[sizeof(T) * 2]) {
+    if (row >= p.M || col0 >= p.N) return;
+    const T* at = static_cast<const T*>(p.C) + uint64_t(row) * p.ldc + col0;
+    if (p.vec_c && col0 + 32 <= p.N) {
+#pragma unroll
+        for (int u = 0; u < int(sizeof(T)) * 2; ++u) c[u] = reinterpret_cast<const uint4*>(at)[u];
+    } else {
+        T* e = reinterpret_cast<T*>(&c);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) e[i] = col0 + i < p.N ? at[i] : T(0.f);
+    }
+}
+
+// 32 finished columns col0.. of `row`, scaled by sa * sb[0..31], (+ beta * C), to the staging row (16-byte units unit0..,
+// swizzled) or to D
 template <typename T>
 __device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t row, uint32_t col0, const uint32_t (&v)[32], float sa,
-                                               const float* sb, uint32_t stage_row, uint32_t unit0, bool c_staged) {
+                                               const float* sb, const uint4 (&c)[sizeof(T) * 2], uint32_t stage_row, uint32_t unit0) {
     constexpr int PER = 16 / sizeof(T);                               // elements per 16-byte unit
     const uint32_t ncols = min(32u, p.N - col0), sw = (stage_row >> 7) & 7u;
-    const bool has_c = p.C != nullptr && row < p.M;
     T* drow = static_cast<T*>(p.D) + uint64_t(row) * p.ldd + col0;
-    const T* crow = has_c ? static_cast<const T*>(p.C) + uint64_t(row) * p.ldc + col0 : nullptr;
 #pragma unroll
     for (int u = 0; u < 32 / PER; ++u) {
         float d[PER];
@@ -331,28 +345,21 @@ __device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t r
             d[i + 2] = __uint_as_float(v[u * PER + i + 2]) * (sa * b.z);
             d[i + 3] = __uint_as_float(v[u * PER + i + 3]) * (sa * b.w);
         }
-        if (has_c) {
-            if (c_staged) {
-                const uint4 c4 = ld_shared_v4(stage_row + (((unit0 + u) ^ sw) << 4));
-                const T* c = reinterpret_cast<const T*>(&c4);
+        if (p.C != nullptr) {
+            const T* e = reinterpret_cast<const T*>(&c[u]);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) d[i] = fmaf(p.beta, q8_to_f32(c[i]), d[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (u * PER + i < ncols) d[i] = fmaf(p.beta, q8_to_f32(crow[u * PER + i]), d[i]);
-            }
+            for (int i = 0; i < PER; ++i) d[i] = fmaf(p.beta, q8_to_f32(e[i]), d[i]);
         }
-        if (stage_row != 0) {
-            uint4 o;
-            T* e = reinterpret_cast<T*>(&o);
+        uint4 o;
+        T* e = reinterpret_cast<T*>(&o);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) q8_put(e + i, d[i]);
+        for (int i = 0; i < PER; ++i) q8_put(e + i, d[i]);
+        if (stage_row != 0) {
             st_shared_v4(stage_row + (((unit0 + u) ^ sw) << 4), o.x, o.y, o.z, o.w);
-        } else {
+        } else if (row < p.M) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (u * PER + i < ncols) q8_put(drow + u * PER + i, d[i]);
+                if (u * PER + i < ncols) drow[u * PER + i] = e[i];
         }
     }
 }
@@ -360,13 +367,13 @@ __device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t r
 template <typename T>
 __global__ void __launch_bounds__(PairCfg::THREADS, 1)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmC, const GemmQ8Params p) {
+                    const __grid_constant__ CUtensorMap tmD, const GemmQ8Params p) {
     constexpr int STAGES = PairCfg::STAGES;
     extern __shared__ uint8_t q8_smem[];
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
     const uint32_t staging = base + STAGES * PairCfg::STAGE;
     const uint32_t full = staging + PairCfg::STAGING, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, acce = accf + 16;
-    const uint32_t cbar0 = acce + 16, slot = cbar0 + 8 * PairCfg::EPI_WARPS;
+    const uint32_t slot = acce + 16;
     uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
     float* const sb_tile = reinterpret_cast<float*>(smem + (full + 256 - base));       // the tile's 256 scales of B
 
@@ -386,7 +393,6 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             mbar_init(accf + 8 * a, 1);
             mbar_init(acce + 8 * a, 2 * PairCfg::EPI_WARPS);          // the epilogue warps of both CTAs
         }
-        for (int w = 0; w < PairCfg::EPI_WARPS; ++w) mbar_init(cbar0 + 8 * w, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -485,17 +491,18 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         // TMA clips a column edge in 16-byte units: a box that crosses an edge N which is not 16-byte aligned is
         // written by predicated per-thread stores
         const bool ragged = ((p.N * uint32_t(sizeof(T))) & 15u) != 0u;
-        const uint32_t cbar = cbar0 + 8 * (warp - 2u);
-        uint32_t cph = 0, it = 0;
+        uint32_t it = 0;
         bool ok = true;
         for (uint32_t t = worker; t < n_tiles; t += workers, ++it) {
             uint32_t tm, tn;
             q8_tile_coords(t, p, tm, tn);
-            const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane;
+            const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane, colbase = tn * 256 + half * 128;
             const float sa = row < p.M ? p.alpha * p.sa[row] : 0.f;
-            // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more
+            // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more, and C
             const uint32_t sb_col = tn * 256 + threadIdx.x - 64;
             const float sb_mine = sb_col < p.N ? __ldg(p.sb + sb_col) : 0.f;
+            uint4 cbuf[2][sizeof(T) * 2];
+            if (p.C != nullptr) q8_load_c<T>(p, row, colbase, cbuf[0]);
             asm volatile("bar.sync 1, 256;" ::: "memory");
             sb_tile[threadIdx.x - 64] = sb_mine;
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -506,44 +513,28 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             tc_fence_after_sync();
             const uint32_t taddr = tmem + a * 256 + half * 128 + ((quarter * 32u) << 16);
-#pragma unroll 1
-            for (uint32_t c = 0; c < 4 && ok; ++c) {
-                const uint32_t col0 = tn * 256 + half * 128 + c * 32;
-                if (col0 >= p.N) break;
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {
+                const uint32_t col0 = colbase + c * 32;
+                if (!ok || col0 >= p.N) break;
+                if (p.C != nullptr && c < 3) q8_load_c<T>(p, row, col0 + 32, cbuf[(c + 1) & 1]);
                 uint32_t v[32];
                 tmem_ld_32x32(taddr + c * 32, v);
                 tmem_ld_wait();
                 const uint32_t sub = c & (SUB - 1), box0 = col0 - sub * 32;
-                if (p.d_tma && !(ragged && box0 + BOX > p.N)) {
-                    const bool c_box = p.c_tma && warp_row0 < p.M;
-                    if (sub == 0) {
-                        if (lane == 0) bulk_wait_read_all();          // the previous box has left the staging tile
-                        __syncwarp();
-                        if (c_box) {
-                            if (lane == 0) {
-                                mbar_arrive_expect_tx(cbar, 4096u);
-                                tma_load_2d(stage_warp, &tmC, cbar, int32_t(box0), int32_t(warp_row0));
-                            }
-                            const bool got = mbar_wait_bounded(cbar, cph, limit);
-                            cph ^= 1u;
-                            if (!got) {
-                                if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-                                ok = false;
-                                break;
-                            }
-                        }
+                const bool boxed = p.d_tma && !(ragged && box0 + BOX > p.N);
+                if (boxed && sub == 0) {
+                    if (lane == 0) bulk_wait_read_all();              // the previous box has left the staging tile
+                    __syncwarp();
+                }
+                q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + half * 128 + c * 32, cbuf[c & 1], boxed ? stage_row : 0u, sub * (8 / SUB));
+                if (boxed && (sub == SUB - 1 || col0 + 32 >= p.N)) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && warp_row0 < p.M) {
+                        tma_store_2d(&tmD, stage_warp, int32_t(box0), int32_t(warp_row0));
+                        bulk_commit_group();
                     }
-                    q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + (col0 - tn * 256), stage_row, sub * (8 / SUB), c_box);
-                    if (sub == SUB - 1 || col0 + 32 >= p.N) {
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0 && warp_row0 < p.M) {
-                            tma_store_2d(&tmD, stage_warp, int32_t(box0), int32_t(warp_row0));
-                            bulk_commit_group();
-                        }
-                    }
-                } else if (row < p.M) {
-                    q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + (col0 - tn * 256), 0, 0, false);
                 }
             }
             tc_fence_before_sync();

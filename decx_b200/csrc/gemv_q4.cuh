@@ -1,26 +1,28 @@
 // Matrix-vector products with 4-bit weights: y[v][r] = xs[v] * sum_g s[r][g] * sum_{k in g} (q[r][k] - z[r][g]) * x[v][k]
 // for 1 to 16 vectors at once.
 //
-// The weights are read once and set the pace (HBM), so the kernel is built around having enough of them in flight:
-//   * A CTA owns 64 rows and a slice of K (512, 1024 or 2048 weights of each row, 16 to 64 KB).  It asks for the whole
-//     slice at once with 16-byte asynchronous copies into shared memory, stages x and the scales while they fly, and
-//     several CTAs share an SM, so that one computes while others wait.  No ring, no waits that could expire.
-//   * The CTAs of a row block's slices form a cluster and add their partial sums through distributed shared memory, in
-//     slice order: one launch, no workspace, no atomics, the same result every time.
-//   * The products run on the warp-level tensor path, m16n8k16 with fp32 accumulators: 16 rows times up to 8 vectors
-//     per instruction, for the price of one vector.  tcgen05 would need the unpacked weights in shared memory, which
-//     costs more than the arithmetic.
+// The weights are read once and set the pace (HBM).  The kernel gives every warp a piece of K that never changes, 256
+// columns (128 for more than eight vectors), and lets it walk down the rows:
+//   * its part of x sits in registers for the whole launch, already in the order the products want;
+//   * weights stream through a ring of 16-row tiles in shared memory that belongs to the warp alone, filled by 16-byte
+//     asynchronous copies: no barrier between copying and multiplying, and no wait that could expire;
+//   * the warps of a CTA (up to 16) cover neighbouring pieces of K and, every 16 to 64 rows, add their partial sums
+//     through shared memory; up to eight CTAs of a cluster do so through distributed shared memory, one round later, so
+//     that nobody waits for the slowest.  Fixed order, no atomics, one launch, no workspace.
+// The products run on the warp-level tensor path, m16n8k16 with fp32 accumulators: 16 rows times up to 8 vectors per
+// instruction, for the price of one vector.  tcgen05 would need unpacked weights in shared memory, which costs more than
+// the arithmetic.
+//
 // Exactness and cost.  A nibble q left in the low bits of an fp16 number IS the subnormal q * 2^-24 (16 q * 2^-24 for the
 // upper nibble of a byte), and the tensor path multiplies subnormals exactly: one mask per pair of weights is all the
 // unpacking there is.  Products of lower and of upper nibbles go to accumulators of their own, and the zero point
-// leaves the sum: sum (q - z) x = sum q x - z sum x, with the group sums of x computed once per CTA.  x is fp16 or e4m3,
-// which fp16 holds exactly.  All sums are fp32; the group's scale multiplies in fp32; the only other rounding is the
-// one to an fp16 result.
+// leaves the sum: sum (q - z) x = sum q x - z sum x, with the group sums of x computed once.  x is fp16 or e4m3, which
+// fp16 holds exactly.  All sums are fp32; the group's scale multiplies in fp32; 2^24 comes back at the end; the only
+// other rounding is the one to an fp16 result.
 //
 // Order of K.  A sum does not care, so each lane takes whole words of a row: of a group of 32 / 64 / 128 weights the lane
 // that the instruction gives columns 2t, 2t+1, 2t+8, 2t+9 holds words t*w .. t*w+w-1 (w = 1 / 2 / 4, one shared-memory
-// load), and x is staged in shared memory in the order that this and the masks produce (0 4 2 6 1 5 3 7 within eight),
-// so that one 16-byte load feeds both instructions of a word.
+// load), and its registers hold the matching x as 0 4 2 6 1 5 3 7 within eight.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -39,40 +41,30 @@ struct GemvQ4Params {
     void* y;                   // n_vec x rows
     uint64_t ldw, lds, ldz, ldx, ldy;
     uint32_t rows, cols, n_vec;
-    uint32_t slice;            // weights of a row per CTA and round: 512, 1024 or 2048
-    uint32_t n_slices;
-    uint32_t ranks;            // CTAs of a row block = cluster size, at most 8
-    int vec_s, vec_z;          // four neighbouring scales / zero points may be read at once
+    uint32_t ranks;            // CTAs that share a block of rows = cluster size, at most 8
+    uint32_t passes;           // 1 unless K is longer than ranks * warps pieces
+    uint32_t tiles;            // 16-row tiles per block of rows: 1, 2 or 4
+    int vec_s, vec_z;          // a tile's scales / zero points of one row may be read at once
 };
 
-constexpr int Q4_ROWS = 64;          // rows per CTA
-constexpr int Q4_THREADS = 256;      // 2 row halves x 4 parts of the slice
-
-__host__ __device__ constexpr uint32_t q4_w_pitch(uint32_t slice) { return slice / 2; }
-// fp16 row of x: 64 bytes more than the slice, so that the two rows a quarter-warp reads fall on different banks
-__host__ __device__ constexpr uint32_t q4_x_pitch(uint32_t slice) { return slice * 2 + 64; }
-// a row's scales (fp32, or fp32 pairs with the zero point), padded against bank conflicts
-__host__ __device__ constexpr uint32_t q4_s_pitch(uint32_t groups, bool zeros) { return zeros ? (groups + 2) * 8 : (groups + 4) * 4; }
-__host__ __device__ constexpr uint32_t q4_red_bytes(uint32_t n_tiles) { return 4u * Q4_ROWS * (8 * n_tiles + 1) * 4; }
-__host__ __device__ constexpr uint32_t q4_smem_bytes(uint32_t slice, uint32_t group, uint32_t n_tiles, uint32_t n_vec,
-                                                     bool zeros) {
-    const uint32_t w = Q4_ROWS * q4_w_pitch(slice);
-    const uint32_t x = n_vec * q4_x_pitch(slice);
-    const uint32_t s = Q4_ROWS * q4_s_pitch(slice / group, zeros);
-    const uint32_t sums = slice / group * 8 * n_tiles * 4;                    // group sums of x
-    const uint32_t red = q4_red_bytes(n_tiles) + Q4_ROWS * 8 * n_tiles * 4;   // reuses the weights' and x's space
-    const uint32_t total = w + x + s + sums;
-    return total > red ? total : red;
-}
-// 16-byte unit u of row r lies at unit u ^ q4_swizzle(r): loads of 4, 8 and 16 bytes per lane, eight rows by four
-// lanes, then meet no bank twice (bit-reversed row number within eight)
-__host__ __device__ constexpr uint32_t q4_swizzle(uint32_t r) { return ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1); }
+template <int NT>
+struct Q4Cfg {
+    static constexpr int KW = NT == 1 ? 256 : 128;            // columns of a warp
+    static constexpr int UNITS = KW / 32;                     // 16-byte units of a row of a tile
+    static constexpr uint32_t TILE = 16 * UNITS * 16;         // bytes
+    static constexpr int STAGES = NT == 1 ? 4 : 8;            // 8 KB per warp
+    static constexpr int MAX_TILES = NT == 1 ? 4 : 2;
+    static constexpr int RS = 16 * MAX_TILES + 4;             // floats between vectors: no bank twice
+    static constexpr int WARPS = 16;                          // most per CTA
+    static constexpr uint32_t PART = 8 * NT * RS * 4;         // bytes of one warp's partial sums
+    static constexpr uint32_t SUMS = 8 * NT * 16 * MAX_TILES * 4;
+    static constexpr uint32_t smem(uint32_t warps) { return warps * (STAGES * TILE + 2 * PART) + 2 * SUMS; }
+};
+static_assert(Q4Cfg<1>::smem(16) <= 227 * 1024 && Q4Cfg<2>::smem(16) <= 227 * 1024, "one CTA's shared memory");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
@@ -93,6 +85,7 @@ __device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ float half_bits(uint32_t u) { return __half2float(__ushort_as_half(uint16_t(u))); }
 
 // W words (1, 2 or 4) from shared memory
 template <int W>
@@ -107,250 +100,318 @@ __device__ __forceinline__ void q4_words(uint32_t at, uint32_t (&w)[W]) {
     }
 }
 
+// 16-byte unit u of row r of a tile lies at unit u ^ q4_swizzle(r): loads of 4, 8 and 16 bytes per lane, eight rows by
+// four lanes, then meet no bank twice (bits of the row number reversed; with rows of 64 bytes, two of them share a line)
+template <int UNITS>
+__host__ __device__ constexpr uint32_t q4_swizzle(uint32_t r) {
+    return UNITS == 8 ? ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
+}
+
+// BYTES consecutive bytes (1, 2, 4, 8 or 16) from a naturally aligned address, as words
+template <int BYTES>
+__device__ __forceinline__ void q4_load_bytes(const void* p, uint32_t (&w)[(BYTES + 3) / 4]) {
+    if constexpr (BYTES == 1) w[0] = __ldg(static_cast<const uint8_t*>(p));
+    else if constexpr (BYTES == 2) w[0] = __ldg(static_cast<const uint16_t*>(p));
+    else if constexpr (BYTES == 4) w[0] = __ldg(static_cast<const uint32_t*>(p));
+    else if constexpr (BYTES == 8) { const uint2 v = __ldg(static_cast<const uint2*>(p)); w[0] = v.x; w[1] = v.y; }
+    else { const uint4 v = __ldg(static_cast<const uint4*>(p)); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+}
+
 template <typename OUT>
 __device__ __forceinline__ OUT q4_out(float v);
 template <> __device__ __forceinline__ float q4_out<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half q4_out<__half>(float v) { return __float2half_rn(v); }
 
-// NT: tiles of eight vectors (1 or 2).  X8: x is e4m3.  grid = row blocks x ranks, ranks innermost (a cluster).
+// Eight entries of x as four fp16 pairs (0,1) (2,3) (4,5) (6,7); zeros behind the last column
+template <bool X8>
+__device__ __forceinline__ void q4_load_x(const GemvQ4Params& p, uint32_t v, uint32_t k, uint32_t (&e)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = 0u;
+    if (v >= p.n_vec || k >= p.cols) return;
+    if constexpr (X8) {
+        const uint8_t* src = static_cast<const uint8_t*>(p.x) + uint64_t(v) * p.ldx + k;
+        uint32_t b[2] = {0u, 0u};
+        if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+            q4_load_bytes<8>(src, b);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (k + j < p.cols) b[j >> 2] |= uint32_t(src[j]) << (8 * (j & 3));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint16_t two = uint16_t(b[j >> 1] >> (16 * (j & 1)));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(e[j]) : "h"(two));
+        }
+    } else {
+        const __half* src = static_cast<const __half*>(p.x) + uint64_t(v) * p.ldx + k;
+        if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            q4_load_bytes<16>(src, e);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (k + j < p.cols) e[j >> 1] |= uint32_t(__half_as_ushort(src[j])) << (16 * (j & 1));
+        }
+    }
+}
+
+// NT: tiles of eight vectors (1 or 2).  X8: x is e4m3.  grid = clusters x ranks, ranks innermost; a cluster takes every
+// (gridDim.x / ranks)-th block of rows.
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
-__global__ void __launch_bounds__(Q4_THREADS)
+__global__ void __launch_bounds__(32 * Q4Cfg<NT>::WARPS, 1)
 gemv_q4_kernel(const GemvQ4Params p) {
-    extern __shared__ __align__(128) uint8_t q4_smem[];      // the swizzle works on address bits 4 to 6
+    using Cfg = Q4Cfg<NT>;
+    constexpr int KW = Cfg::KW, UNITS = Cfg::UNITS, STAGES = Cfg::STAGES, RS = Cfg::RS;
     constexpr int WPL = GROUP / 32;                           // words a lane holds of a row's group
-    constexpr int GU = GROUP / 8;                             // 16-byte units of x in a group
-    constexpr int NV = 8 * NT;
-    const uint32_t base = smem_u32(q4_smem);
-    const uint32_t wp = q4_w_pitch(p.slice), xp = q4_x_pitch(p.slice);
-    const uint32_t gps = p.slice / GROUP, gps_log = 31 - __clz(gps), s_pitch = q4_s_pitch(gps, ZEROS);
-    const uint32_t x_off = Q4_ROWS * wp, s_off = x_off + p.n_vec * xp, xs_off = s_off + Q4_ROWS * s_pitch;
+    constexpr int GC = KW / GROUP;                            // groups of a warp's piece
+    constexpr uint32_t PITCH = UNITS * 16;
+    extern __shared__ __align__(128) uint8_t q4_smem[];      // the swizzle works on address bits 4 to 6
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t half = warp & 1, part = warp >> 1;         // rows [32 half, +32), quarter `part` of the slice
-    const uint32_t ranks = p.ranks, rank = blockIdx.x % ranks;
-    const uint32_t row0 = blockIdx.x / ranks * Q4_ROWS;
-    const uint32_t row_bytes = (p.cols + 1) / 2;
+    const uint32_t warps = blockDim.x >> 5, ranks = p.ranks, rank = blockIdx.x % ranks;
+    const uint32_t cluster_id = blockIdx.x / ranks, clusters = gridDim.x / ranks;
+    const uint32_t R = 16 * p.tiles, blocks = (p.rows + R - 1) / R;
+    const uint32_t row_bytes = (p.cols + 1) / 2, groups = (p.cols + GROUP - 1) / GROUP;
+    const uint32_t pieces = (p.cols + KW - 1) / KW;
+    const uint32_t ring = smem_u32(q4_smem) + warp * STAGES * Cfg::TILE;
+    float* const parts = reinterpret_cast<float*>(q4_smem + warps * STAGES * Cfg::TILE);      // [2][warp][vector][RS]
+    float* const sums = parts + 2 * warps * (Cfg::PART / 4);                                  // [2][vector][R]
+    // pieces this CTA covers in pass 0 (later passes have at most as many: their missing warps add nothing)
+    const uint32_t piece0 = rank * warps + warp, pass_step = ranks * warps;
+    const uint32_t active = min(warps, pieces > rank * warps ? pieces - rank * warps : 0u);
 
-    float acc[2][NT][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-
-    for (uint32_t sl = rank; sl < p.n_slices; sl += ranks) {
-        const uint32_t k0 = sl * p.slice;
-        const uint32_t kn = min(p.slice, p.cols - k0);        // weights of a row in this slice
-        const uint32_t gn = (kn + GROUP - 1) / GROUP;         // its groups; the last one may be short
-        if (sl != rank) __syncthreads();                      // the previous slice has been consumed
-        // ---- weights: warp w brings rows 8w .. 8w+7, a lane every 32nd 16-byte unit.  Bytes behind the row's end and
-        // rows behind the last one become zeros.
-        for (uint32_t u = lane; u < gn * (GROUP / 32); u += 32) {
-            const uint32_t byte = k0 / 2 + u * 16;
+    // ---- the stream of tiles: blocks, passes over K within a block, tiles within a pass
+    const uint32_t my_blocks = blocks > cluster_id ? (blocks - cluster_id - 1) / clusters + 1 : 0u;
+    const uint32_t n_tiles = my_blocks * p.passes * p.tiles;
+    const uint32_t lrow = lane / UNITS, lunit = lane % UNITS; // this lane's first unit of a tile; the others 32 / UNITS rows on
+    uint32_t rq_i = 0, rq_tile = 0, rq_pass = 0, rq_block = cluster_id, rq_stage = 0;
+    auto request = [&]() {
+        const uint32_t piece = piece0 + rq_pass * pass_step;
+        if (rq_i < n_tiles && piece < pieces) {
+            const uint32_t row0 = rq_block * R + rq_tile * 16 + lrow, byte = piece * (KW / 2) + lunit * 16;
             const uint32_t n = byte < row_bytes ? min(16u, row_bytes - byte) : 0u;
-            const uint8_t* src = p.W + uint64_t(row0 + warp * 8) * p.ldw + byte;
-            const uint32_t dst = base + warp * 8 * wp + u * 16;
+            const uint8_t* src = p.W + uint64_t(row0) * p.ldw + byte;
+            const uint32_t dst = ring + rq_stage * Cfg::TILE + lrow * PITCH;
 #pragma unroll
-            for (uint32_t r = 0; r < 8; ++r) {
-                const bool in = n != 0 && row0 + warp * 8 + r < p.rows;
-                cp_async16((dst ^ (q4_swizzle(r) * 16)) + r * wp, in ? src : p.W, in ? n : 0u);
-                src += p.ldw;
+            for (uint32_t i = 0; i < 16u * UNITS / 32; ++i) {
+                constexpr uint32_t ROWS = 32 / UNITS;         // rows per instruction
+                const bool in = n != 0 && row0 + i * ROWS < p.rows;
+                cp_async16(dst + i * ROWS * PITCH + ((lunit ^ q4_swizzle<UNITS>(lrow + i * ROWS)) * 16), in ? src : p.W, in ? n : 0u);
+                src += ROWS * p.ldw;
             }
         }
-        // ---- x as fp16 in the order of the products, zeros behind the last column, and the sums of its groups
-        for (uint32_t v = 0; v < p.n_vec; ++v) {
-            for (uint32_t u = threadIdx.x; u < gps * GU; u += Q4_THREADS) {      // a multiple of 32: whole warps
-                const uint32_t k = k0 + u * 8;
-                uint32_t e[4];                                // pairs (0,1) (2,3) (4,5) (6,7)
-                if constexpr (X8) {
-                    const uint8_t* src = static_cast<const uint8_t*>(p.x) + uint64_t(v) * p.ldx + k;
-                    uint32_t b[2] = {0u, 0u};
-                    if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 7) == 0) {
-                        const uint2 d = *reinterpret_cast<const uint2*>(src);
-                        b[0] = d.x;
-                        b[1] = d.y;
-                    } else if (k < p.cols) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (k + j < p.cols) b[j >> 2] |= uint32_t(src[j]) << (8 * (j & 3));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint16_t two = uint16_t(b[j >> 1] >> (16 * (j & 1)));
-                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(e[j]) : "h"(two));
-                    }
-                } else {
-                    const __half* src = static_cast<const __half*>(p.x) + uint64_t(v) * p.ldx + k;
-                    if (k + 8 <= p.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                        const uint4 d = *reinterpret_cast<const uint4*>(src);
-                        e[0] = d.x; e[1] = d.y; e[2] = d.z; e[3] = d.w;
-                    } else {
-                        __half h[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) h[j] = k + j < p.cols ? src[j] : __float2half(0.f);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = h2_bits(__halves2half2(h[2 * j], h[2 * j + 1]));
-                    }
-                }
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = __half22float2(bits_h2(e[j]));
-                    sum += f.x + f.y;
-                }
-#pragma unroll
-                for (int m = 1; m < GU; m *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-                const uint32_t gi = u / GU, w = u % GU;       // word w of the group belongs to lane w / WPL
-                if (w == 0) *reinterpret_cast<float*>(q4_smem + xs_off + (gi * NV + v) * 4) = sum * 0x1p-24f;
-                st_shared_v4(base + x_off + v * xp + (gi * GU + (w % WPL) * 4 + w / WPL) * 16,
-                             __byte_perm(e[0], e[2], 0x5410), __byte_perm(e[1], e[3], 0x5410),
-                             __byte_perm(e[0], e[2], 0x7632), __byte_perm(e[1], e[3], 0x7632));
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++rq_i;
+        if (++rq_stage == STAGES) rq_stage = 0;
+        if (++rq_tile == p.tiles) {
+            rq_tile = 0;
+            if (++rq_pass == p.passes) {
+                rq_pass = 0;
+                rq_block += clusters;
             }
         }
-        // ---- scales (times 2^24) and zero points (negative), four neighbouring groups at a time
-        const uint32_t g0 = k0 / GROUP;
-        for (uint32_t i = threadIdx.x; i < Q4_ROWS * gps / 4; i += Q4_THREADS) {
-            const uint32_t r = i >> (gps_log - 2), gi = (i & (gps / 4 - 1)) * 4;
-            if (gi >= gn || row0 + r >= p.rows) continue;
-            const __half* sp = p.scales + uint64_t(row0 + r) * p.lds + g0 + gi;
-            float s[4], z[4];
-            if (p.vec_s && gi + 4 <= gn) {
-                const uint2 d = *reinterpret_cast<const uint2*>(sp);
-                const float2 a = __half22float2(bits_h2(d.x)), b = __half22float2(bits_h2(d.y));
-                s[0] = a.x; s[1] = a.y; s[2] = b.x; s[3] = b.y;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] = gi + j < gn ? __half2float(sp[j]) : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] *= 0x1p24f;
-            const uint32_t at = base + s_off + r * s_pitch + gi * (ZEROS ? 8 : 4);
-            if constexpr (ZEROS) {
-                const uint8_t* zp = p.zeros + uint64_t(row0 + r) * p.ldz + g0 + gi;
-                if (p.vec_z && gi + 4 <= gn) {
-                    const uint32_t d = *reinterpret_cast<const uint32_t*>(zp);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) z[j] = -float((d >> (8 * j)) & 255u);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) z[j] = gi + j < gn ? -float(zp[j]) : 0.f;
-                }
-                st_shared_v4(at, __float_as_uint(s[0]), __float_as_uint(z[0]), __float_as_uint(s[1]), __float_as_uint(z[1]));
-                st_shared_v4(at + 16, __float_as_uint(s[2]), __float_as_uint(z[2]), __float_as_uint(s[3]), __float_as_uint(z[3]));
-            } else {
-                st_shared_v4(at, __float_as_uint(s[0]), __float_as_uint(s[1]), __float_as_uint(s[2]), __float_as_uint(s[3]));
-            }
-        }
-        cp_async_wait_all();
-        __syncthreads();
+    };
+    for (int d = 0; d < STAGES - 1; ++d) request();
 
-        // ---- multiply: this warp's 32 rows, its quarter of the slice's groups
-        const uint32_t per = (gn + 3) / 4, gi1 = min(gn, (part + 1) * per);
-        const uint32_t wrow = base + (half * 32 + g) * wp, sw = q4_swizzle(g) * 16;   // rows 8 apart share a swizzle
-        uint32_t xv[NT];                                      // lanes of vectors that do not exist read the last one;
-#pragma unroll                                                // their columns are never stored
-        for (int n = 0; n < NT; ++n) xv[n] = base + x_off + min(uint32_t(n * 8) + g, p.n_vec - 1) * xp + t * 16;
-#pragma unroll 1
-        for (uint32_t gi = part * per; gi < gi1; ++gi) {
-            uint32_t w[4][WPL];
+    // ---- scales and zero points of rows g and g + 8 of a tile, asked for one tile ahead
+    uint32_t sraw[2][(2 * GC + 3) / 4], zraw[2][(GC + 3) / 4];
+    uint32_t sq_tile = 0, sq_pass = 0, sq_block = cluster_id, sq_i = 0;
+    auto request_scales = [&]() {
+        const uint32_t g0 = (piece0 + sq_pass * pass_step) * GC;
+        if (sq_i < n_tiles && g0 < groups) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m) q4_words<WPL>(wrow + m * 8 * wp + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), w[m]);
-            float lo[2][NT][4], hi[2][NT][4];
+            for (int h = 0; h < 2; ++h) {
+                // rows behind the last one repeat it: their sums are never stored
+                const uint64_t row = min(sq_block * R + sq_tile * 16 + h * 8 + g, p.rows - 1);
+                const __half* sp = p.scales + row * p.lds + g0;
+                if (p.vec_s && g0 + GC <= groups) {
+                    q4_load_bytes<2 * GC>(sp, sraw[h]);
+                } else {
 #pragma unroll
-            for (int j = 0; j < WPL; ++j) {
-                uint4 xb[NT];
+                    for (int j = 0; j < GC; ++j) {
+                        const uint32_t b = g0 + j < groups ? __half_as_ushort(sp[j]) : 0u;
+                        sraw[h][j / 2] = (j & 1) ? (sraw[h][j / 2] | (b << 16)) : b;
+                    }
+                }
+                if constexpr (ZEROS) {
+                    const uint8_t* zp = p.zeros + row * p.ldz + g0;
+                    if (p.vec_z && g0 + GC <= groups) {
+                        q4_load_bytes<GC>(zp, zraw[h]);
+                    } else {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) xb[n] = ld_shared_v4(xv[n] + (gi * GU + j * 4) * 16);
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    const uint32_t wa = w[2 * m][j], wb = w[2 * m + 1][j], wa8 = wa >> 8, wb8 = wb >> 8;
-                    constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (j == 0) {
-                            mma_16816_first(lo[m][n], wa & L, wb & L, wa8 & L, wb8 & L, xb[n].x, xb[n].y);
-                            mma_16816_first(hi[m][n], wa & H, wb & H, wa8 & H, wb8 & H, xb[n].z, xb[n].w);
-                        } else {
-                            mma_16816(lo[m][n], wa & L, wb & L, wa8 & L, wb8 & L, xb[n].x, xb[n].y);
-                            mma_16816(hi[m][n], wa & H, wb & H, wa8 & H, wb8 & H, xb[n].z, xb[n].w);
+                        for (int j = 0; j < GC; ++j) {
+                            const uint32_t b = g0 + j < groups ? zp[j] : 0u;
+                            zraw[h][j / 4] = (j & 3) ? (zraw[h][j / 4] | (b << (8 * (j & 3)))) : b;
                         }
                     }
                 }
             }
-            float sc[4], nz[4];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const uint32_t at = base + s_off + (half * 32 + m * 8 + g) * s_pitch + gi * (ZEROS ? 8 : 4);
-                if constexpr (ZEROS) {
-                    uint32_t v[2];
-                    q4_words<2>(at, v);
-                    sc[m] = __uint_as_float(v[0]);
-                    nz[m] = __uint_as_float(v[1]);
-                } else {
-                    sc[m] = __uint_as_float(ld_shared_u32(at));
-                    nz[m] = -8.f;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uint32_t v[2];
-                q4_words<2>(base + xs_off + (gi * NV + n * 8 + 2 * t) * 4, v);
-                const float xs[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {             // i >> 1: row g or g + 8; i & 1: vector 2t or 2t + 1
-                        float d = fmaf(hi[m][n][i], 0.0625f, lo[m][n][i]);
-                        d = fmaf(nz[2 * m + (i >> 1)], xs[i & 1], d);
-                        acc[m][n][i] = fmaf(sc[2 * m + (i >> 1)], d, acc[m][n][i]);
-                    }
-            }
         }
-    }
-
-    // ---- join: the four quarters through shared memory, then the slices through distributed shared memory
-    __syncthreads();
-    constexpr int RP = NV + 1;
-    float* red = reinterpret_cast<float*>(q4_smem);                       // [part][row][RP]
-    float* sums = red + 4 * Q4_ROWS * RP;                                 // [vector][row]
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t r = half * 32 + m * 16 + g + (i >> 1) * 8, v = n * 8 + 2 * t + (i & 1);
-                if (v < p.n_vec) red[(part * Q4_ROWS + r) * RP + v] = acc[m][n][i];
+        ++sq_i;
+        if (++sq_tile == p.tiles) {
+            sq_tile = 0;
+            if (++sq_pass == p.passes) {
+                sq_pass = 0;
+                sq_block += clusters;
             }
-    __syncthreads();
-    auto store = [&](uint32_t v, uint32_t r, float s) {
-        if (row0 + r < p.rows) {
-            if (p.xs != nullptr) s *= __ldg(p.xs + v);
-            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row0 + r] = q4_out<OUT>(s);
         }
     };
-    for (uint32_t i = threadIdx.x; i < Q4_ROWS * p.n_vec; i += Q4_THREADS) {
-        const uint32_t v = i / Q4_ROWS, r = i % Q4_ROWS;
-        float s = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s += red[(q * Q4_ROWS + r) * RP + v];
-        if (ranks > 1) sums[i] = s;
-        else store(v, r, s);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < (2 * GC + 3) / 4; ++j) sraw[h][j] = 0u;
+#pragma unroll
+        for (int j = 0; j < (GC + 3) / 4; ++j) zraw[h][j] = 0u;
     }
-    if (ranks > 1) {
+    request_scales();
+
+    // ---- this warp's x: registers in product order, and the group sums of the vectors whose columns this lane gets
+    uint4 xr[GC * WPL][NT];
+    float xsum[GC][NT][2];
+    auto load_x = [&](uint32_t piece) {
+#pragma unroll
+        for (int gi = 0; gi < GC; ++gi)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < WPL; ++j) {
+                    uint32_t e[4];
+                    q4_load_x<X8>(p, n * 8 + g, piece * KW + gi * GROUP + (t * WPL + j) * 8, e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = __half22float2(bits_h2(e[i]));
+                        sum += f.x + f.y;
+                    }
+                    xr[gi * WPL + j][n] = make_uint4(__byte_perm(e[0], e[2], 0x5410), __byte_perm(e[1], e[3], 0x5410),
+                                                     __byte_perm(e[0], e[2], 0x7632), __byte_perm(e[1], e[3], 0x7632));
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= 0x1p-24f;
+                xsum[gi][n][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                xsum[gi][n][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            }
+    };
+    if (p.passes == 1) load_x(piece0);
+
+    auto store = [&](uint32_t block, uint32_t i, float s) {   // i = vector * R + row
+        const uint32_t v = i / R, row = block * R + i % R;
+        if (row < p.rows) {
+            s *= 0x1p24f;
+            if (p.xs != nullptr) s *= __ldg(p.xs + v);
+            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row] = q4_out<OUT>(s);
+        }
+    };
+    auto join_cluster = [&](uint32_t block, uint32_t buf) {   // all CTAs' sums of a block: requested together, added in order
         namespace cg = cooperative_groups;
         const cg::cluster_group cluster = cg::this_cluster();
-        cluster_sync_all();
-        for (uint32_t i = rank * Q4_THREADS + threadIdx.x; i < Q4_ROWS * p.n_vec; i += ranks * Q4_THREADS) {
-            float d[8];                                                   // requested together, added in slice order
+        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < R * p.n_vec; i += ranks * blockDim.x) {
+            float d[8];
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) d[c] = c < ranks ? *cluster.map_shared_rank(sums + i, c) : 0.f;
+            for (uint32_t c = 0; c < 8; ++c)
+                d[c] = c < ranks ? *cluster.map_shared_rank(sums + buf * (Cfg::SUMS / 4) + i, c) : 0.f;
             float s = 0.f;
 #pragma unroll
             for (uint32_t c = 0; c < 8; ++c) s += d[c];
-            store(i / Q4_ROWS, i % Q4_ROWS, s);
+            store(block, i, s);
         }
-        cluster_sync_all();                                               // nobody leaves while its sums are being read
+    };
+
+    uint32_t stage = 0;
+    const uint32_t sw = q4_swizzle<UNITS>(g) * 16;            // rows g and g + 8 share it
+    for (uint32_t b = 0; b < my_blocks; ++b) {
+        const uint32_t block = cluster_id + b * clusters, buf = b & 1u;
+        float* const part = parts + (buf * warps + warp) * (Cfg::PART / 4);
+        for (uint32_t pass = 0; pass < p.passes; ++pass) {
+            const uint32_t piece = piece0 + pass * pass_step;
+            if (p.passes > 1) load_x(piece);
+            for (uint32_t tile = 0; tile < p.tiles; ++tile) {
+                // the stage that is asked for now was read in the previous turn, by all lanes
+                __syncwarp();
+                request();
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+                __syncwarp();                                 // every lane's copies of this tile have landed
+                float sc[2][GC], nz[2][GC];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < GC; ++j) {
+                        sc[h][j] = half_bits(sraw[h][j / 2] >> (16 * (j & 1)));
+                        if constexpr (ZEROS) nz[h][j] = -float((zraw[h][j / 4] >> (8 * (j & 3))) & 255u);
+                        else nz[h][j] = -8.f;
+                    }
+                request_scales();
+                float acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+                if (piece < pieces) {
+                    const uint32_t wrow = ring + stage * Cfg::TILE + g * PITCH;
+#pragma unroll
+                    for (int gi = 0; gi < GC; ++gi) {
+                        uint32_t wa[WPL], wb[WPL];            // rows g and g + 8
+                        q4_words<WPL>(wrow + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wa);
+                        q4_words<WPL>(wrow + 8 * PITCH + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wb);
+                        float lo[NT][4], hi[NT][4];
+#pragma unroll
+                        for (int j = 0; j < WPL; ++j) {
+                            constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
+                            const uint32_t wa8 = wa[j] >> 8, wb8 = wb[j] >> 8;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint4 x = xr[gi * WPL + j][n];
+                                if (j == 0) {
+                                    mma_16816_first(lo[n], wa[j] & L, wb[j] & L, wa8 & L, wb8 & L, x.x, x.y);
+                                    mma_16816_first(hi[n], wa[j] & H, wb[j] & H, wa8 & H, wb8 & H, x.z, x.w);
+                                } else {
+                                    mma_16816(lo[n], wa[j] & L, wb[j] & L, wa8 & L, wb8 & L, x.x, x.y);
+                                    mma_16816(hi[n], wa[j] & H, wb[j] & H, wa8 & H, wb8 & H, x.z, x.w);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {     // i >> 1: row g or g + 8; i & 1: vector 2t or 2t + 1
+                                float d = fmaf(hi[n][i], 0.0625f, lo[n][i]);
+                                d = fmaf(nz[i >> 1][gi], xsum[gi][n][i & 1], d);
+                                acc[n][i] = fmaf(sc[i >> 1][gi], d, acc[n][i]);
+                            }
+                    }
+                }
+                if (++stage == STAGES) stage = 0;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t v = n * 8 + 2 * t + (i & 1);
+                        float* at = part + v * RS + tile * 16 + g + (i >> 1) * 8;
+                        if (v < p.n_vec) *at = pass == 0 ? acc[n][i] : *at + acc[n][i];
+                    }
+            }
+        }
+        // ---- join.  Two sets of partial sums: what the next block writes is not what this one reads.
+        __syncthreads();
+        if (ranks > 1 && b > 0) {
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            join_cluster(block - clusters, buf ^ 1u);
+        }
+        for (uint32_t i = threadIdx.x; i < R * p.n_vec; i += blockDim.x) {
+            const float* at = parts + buf * warps * (Cfg::PART / 4) + i / R * RS + i % R;
+            float s = 0.f;
+            for (uint32_t w = 0; w < active; ++w) s += at[w * (Cfg::PART / 4)];
+            if (ranks > 1) sums[buf * (Cfg::SUMS / 4) + i] = s;
+            else store(block, i, s);
+        }
+        if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    if (ranks > 1) {
+        if (my_blocks > 0) {
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            join_cluster(cluster_id + (my_blocks - 1) * clusters, (my_blocks - 1) & 1u);
+        }
+        cluster_sync_all();                                   // nobody leaves while its sums are being read
     }
 }
 

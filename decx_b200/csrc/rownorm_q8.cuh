@@ -219,20 +219,16 @@ row_q8_kernel(const RowQ8Params p) {
 
 // ---- ring kernel -------------------------------------------------------------------------------------------
 // Many rows: what limits row_q8_kernel is that a CTA's loads, reduction and stores follow one another (fp16
-// cast of 4096 x 16384: 72 us against 31 us of traffic).  Here the CTAs stay, and every thread asks for its own pieces
-// of the rows to come with asynchronous copies into its own slots of a ring in shared memory.  Nobody else reads a slot,
-// so the ring needs no barrier; the only one per row is the reduction's.
+// cast of 4096 x 16384: 72 us against 31 us of traffic).  Here the CTAs stay, and every thread asks for its own 16-byte
+// units of the rows to come with asynchronous copies into its own slots of a ring in shared memory.  Nobody else reads a
+// slot, so the ring needs no barrier; the only one per row is the reduction's.
 //
-// SHIFT: rows of x, r and sum that start anywhere (an odd row length).  A thread then copies the aligned 16-byte units that
-// its 8 elements touch and shifts them into place; on the way out the lanes of a warp pass each other what an aligned
-// unit of the other side needs.
+// SHIFT: rows of x, r and sum that start anywhere (an odd row length).  The warps then copy the aligned units that their
+// elements touch (33 for 32 lanes), and a lane shifts what it needs out of two of them; on the way out the lanes pass
+// each other what an aligned unit of the other side needs.
 
 __device__ __forceinline__ void q8_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// SHIFT: neighbouring threads ask for overlapping units, so these go through L1
-__device__ __forceinline__ void q8_async16_l1(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void q8_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all but the newest `ahead` groups of this thread have landed
@@ -242,26 +238,27 @@ __device__ __forceinline__ void q8_async_wait(uint32_t ahead) {
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
 
-// N words of `s` from byte `o` (below 16; whole words only when WORDS) on
-template <bool WORDS, int WS, int N, int S>
-__device__ __forceinline__ void q8_pick_at(const uint32_t (&s)[S], uint32_t o, uint32_t (&out)[N]) {
+// four words of `s` from byte `o` (below 16; whole words only when WORDS) on
+template <bool WORDS, int WS>
+__device__ __forceinline__ void q8_pick_at(const uint32_t (&s)[8], uint32_t o, uint32_t (&out)[4]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < 4; ++i) {
         if constexpr (WORDS) out[i] = s[WS + i];
-        else out[i] = __funnelshift_r(s[WS + i], s[WS + i + 1 < S ? WS + i + 1 : S - 1], (o & 2) * 8);
+        else out[i] = __funnelshift_r(s[WS + i], s[WS + i + 1], (o & 2) * 8);
     }
 }
-template <bool WORDS, int N, int S>
-__device__ __forceinline__ void q8_pick(const uint32_t (&s)[S], uint32_t o, uint32_t (&out)[N]) {
+template <bool WORDS>
+__device__ __forceinline__ void q8_pick(const uint32_t (&s)[8], uint32_t o, uint32_t (&out)[4]) {
     switch (o >> 2) {                                     // the same for a whole row
-        case 0: q8_pick_at<WORDS, 0, N, S>(s, o, out); break;
-        case 1: q8_pick_at<WORDS, 1, N, S>(s, o, out); break;
-        case 2: q8_pick_at<WORDS, 2, N, S>(s, o, out); break;
-        default: q8_pick_at<WORDS, 3, N, S>(s, o, out); break;
+        case 0: q8_pick_at<WORDS, 0>(s, o, out); break;
+        case 1: q8_pick_at<WORDS, 1>(s, o, out); break;
+        case 2: q8_pick_at<WORDS, 2>(s, o, out); break;
+        default: q8_pick_at<WORDS, 3>(s, o, out); break;
     }
 }
 
-__device__ __forceinline__ void q8_to_floats(const uint32_t (&w)[4], float (&f)[8], __half) {
+// one 16-byte unit as floats and back
+__device__ __forceinline__ void q8_unit(const uint32_t (&w)[4], float (&f)[8], __half) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -269,47 +266,41 @@ __device__ __forceinline__ void q8_to_floats(const uint32_t (&w)[4], float (&f)[
         f[2 * i + 1] = a.y;
     }
 }
-__device__ __forceinline__ void q8_to_floats(const uint32_t (&w)[8], float (&f)[8], float) {
+__device__ __forceinline__ void q8_unit(const uint32_t (&w)[4], float (&f)[4], float) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void q8_words(const float (&f)[8], uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+__device__ __forceinline__ void q8_words(const float (&f)[4], uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
 }
 
-// 8 elements per lane, consecutive over the warp, to a row that starts anywhere; every lane has all 8
-template <typename T>
-__device__ __forceinline__ void q8_store8_shift(T* at, const float (&f)[8], uint32_t lane) {
-    constexpr int W = 8 * sizeof(T) / 4;                  // words of a lane
-    uint32_t s[W + 4];
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-            s[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __float_as_uint(f[i]);
-    }
+// One unit per lane, consecutive over the warp, to a row that starts anywhere; every lane's unit is whole.
+template <typename T, int E>
+__device__ __forceinline__ void q8_store_shift(T* at, const float (&f)[E], uint32_t lane) {
+    uint32_t s[8], out[4];
+    q8_words(f, s);
     const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
     if (o == 0) {
-#pragma unroll
-        for (int u = 0; u < W / 4; ++u)
-            reinterpret_cast<uint4*>(at)[u] = make_uint4(s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]);
+        *reinterpret_cast<uint4*>(at) = make_uint4(s[0], s[1], s[2], s[3]);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[W + i] = __shfl_down_sync(0xffffffffu, s[i], 1);
+    for (int i = 0; i < 4; ++i) s[4 + i] = __shfl_down_sync(0xffffffffu, s[i], 1);
     const uint32_t d = 16 - o, head = d / sizeof(T);      // the first aligned unit starts this many elements in
-    uint32_t out[W];
-    q8_pick<sizeof(T) == 4, W, W + 4>(s, d, out);
-    uint4* unit = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + d);
+    q8_pick<sizeof(T) == 4>(s, d, out);
+    if (lane < 31) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + d) = make_uint4(out[0], out[1], out[2], out[3]);
+    // what lies before the warp's first and behind its last aligned unit
 #pragma unroll
-    for (int u = 0; u < W / 4; ++u)
-        if (lane < 31 || u + 1 < W / 4) unit[u] = make_uint4(out[4 * u], out[4 * u + 1], out[4 * u + 2], out[4 * u + 3]);
-    // what lies before the warp's first and behind its last whole unit
-    const uint32_t tail = head + 8 * (W / 4 - 1) / (W / 4);
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        if ((lane == 0 && i < head) || (lane == 31 && i >= tail)) q8_store(at + i, f[i]);
+    for (uint32_t i = 0; i < E; ++i)
+        if ((lane == 0 && i < head) || (lane == 31 && i >= head)) q8_store(at + i, f[i]);
 }
 
 template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
@@ -318,77 +309,67 @@ row_q8_ring_kernel(const RowQ8Params p) {
     extern __shared__ __align__(128) uint8_t q8_ring[];
     __shared__ float red_ss[2][32];
     __shared__ uint32_t red_top[2][32];
-    constexpr int U = 8 * sizeof(T) / 16, UL = U + (SHIFT ? 1 : 0);   // 16-byte units of 8 elements, and loaded
-    constexpr int UT = UL * (RES ? 2 : 1);
-    const uint32_t lane = threadIdx.x & 31u;
+    constexpr int E = 16 / sizeof(T), NC = NCH * 8 / E;               // elements of a unit, units of a thread
+    constexpr int MATS = RES ? 2 : 1;
+    const uint32_t lane = threadIdx.x & 31u, wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t tpr = WARP ? 32u : blockDim.x, tid = WARP ? lane : threadIdx.x;
-    const uint32_t step = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
-    const uint32_t first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    const uint32_t unit_step = blockDim.x * 16;                       // a thread's units lie this far apart
-    const uint32_t mine = smem_u32(q8_ring) + threadIdx.x * 16;
+    const uint32_t step = WARP ? gridDim.x * warps : gridDim.x;
+    const uint32_t first = WARP ? blockIdx.x * warps + wid : blockIdx.x;
+    constexpr uint32_t WARP_BYTES = (SHIFT ? 33 : 32) * 16;           // of one warp's units
+    const uint32_t mine = smem_u32(q8_ring) + wid * WARP_BYTES + lane * 16;
     const T* const w = static_cast<const T*>(p.w);
 
-    // ask for this thread's pieces of a row
-    auto request = [&](uint32_t slot, const T* mat, uint64_t ld, uint64_t row, int u0) {
+    auto slot_at = [&](uint32_t slot, int c, int m) { return mine + ((slot * NC + c) * MATS + m) * warps * WARP_BYTES; };
+    // ask for this thread's units of a row
+    auto request = [&](uint32_t slot, const T* mat, uint64_t ld, uint64_t row, int m) {
         const T* const rp = mat + row * ld;
         const uint8_t* const end = reinterpret_cast<const uint8_t*>(rp + p.cols);
+        const uint8_t* const begin = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(rp) & ~uintptr_t(15));
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const uint32_t col = (c * tpr + tid) * 8;
-            if (col >= p.cols) continue;
-            const uint8_t* at = reinterpret_cast<const uint8_t*>(rp + col);
-            const uint32_t dst = mine + ((slot * NCH + c) * UT + u0) * unit_step;
-            if constexpr (SHIFT) {
-                const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
-                at -= o;
-                if (at < reinterpret_cast<const uint8_t*>(mat)) {     // the matrix itself starts inside this unit
-                    T* const own = reinterpret_cast<T*>(q8_ring + (dst - smem_u32(q8_ring)));
+        for (int c = 0; c < NC; ++c) {
+            const uint8_t* at = begin + uint64_t(c * tpr + tid) * 16;
+            const uint32_t dst = slot_at(slot, c, m);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t b = o + i * sizeof(T);         // byte within the units, which lie unit_step apart
-                        own[(b / 16 * unit_step + b % 16) / sizeof(T)] = col + i < p.cols ? rp[col + i] : T(0.f);
-                    }
-                    continue;
+            for (int extra = 0; extra < (SHIFT ? 2 : 1); ++extra) {
+                if (extra == 1) {
+                    if (lane != 31) break;                            // the unit behind the warp's last one
+                    at += 16;
                 }
-                if (o == 0) {                                         // nothing of the last unit is needed
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int64_t left = end - (at + u * 16);
-                        q8_async16_l1(dst + u * unit_step, left > 0 ? at + u * 16 : at, left >= 16 ? 16u : (left > 0 ? uint32_t(left) : 0u));
-                    }
-                    continue;
+                if (at >= end) break;
+                const int64_t left = end - at;
+                if (SHIFT && at < reinterpret_cast<const uint8_t*>(mat)) {
+                    // the matrix itself starts inside this unit: element by element
+                    const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(rp)) & 15u;
+                    T* const own = reinterpret_cast<T*>(q8_ring + (dst - smem_u32(q8_ring)) + o);
+                    for (uint32_t i = 0; i * sizeof(T) + o < 16 && i < p.cols; ++i) own[i] = rp[i];
+                } else {
+                    q8_async16(dst + extra * 16, at, left >= 16 ? 16u : uint32_t(left));
                 }
-            }
-#pragma unroll
-            for (int u = 0; u < UL; ++u) {
-                const int64_t left = end - (at + u * 16);
-                const uint32_t n = left >= 16 ? 16u : (left > 0 ? uint32_t(left) : 0u);
-                if constexpr (SHIFT) q8_async16_l1(dst + u * unit_step, n ? at + u * 16 : at, n);
-                else q8_async16(dst + u * unit_step, n ? at + u * 16 : at, n);
             }
         }
     };
     auto request_row = [&](uint32_t slot, uint64_t row) {
         if (row < p.rows) {
             request(slot, static_cast<const T*>(p.x), p.ldx, row, 0);
-            if constexpr (RES) request(slot, static_cast<const T*>(p.r), p.ldr, row, UL);
+            if constexpr (RES) request(slot, static_cast<const T*>(p.r), p.ldr, row, 1);
         }
         q8_async_commit();
     };
-    auto take = [&](uint32_t slot, int c, const T* mat, uint64_t ld, uint64_t row, int u0, float (&f)[8]) {
-        const uint32_t src = mine + ((slot * NCH + c) * UT + u0) * unit_step;
-        uint32_t s[4 * UL], o4[4 * U];
-#pragma unroll
-        for (int u = 0; u < UL; ++u) {
-            const uint4 v = ld_shared_v4(src + u * unit_step);
-            s[4 * u] = v.x; s[4 * u + 1] = v.y; s[4 * u + 2] = v.z; s[4 * u + 3] = v.w;
-        }
+    // this thread's elements of a unit; what lies behind the row's end is not zero
+    auto take = [&](uint32_t slot, int c, const T* mat, uint64_t ld, uint64_t row, int m, float (&f)[E]) {
+        const uint32_t src = slot_at(slot, c, m);
+        uint32_t s[8], o4[4];
+        const uint4 v = ld_shared_v4(src);
+        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
         if constexpr (SHIFT) {
-            q8_pick<sizeof(T) == 4, 4 * U, 4 * UL>(s, uint32_t(reinterpret_cast<uintptr_t>(mat + row * ld)) & 15u, o4);
-            q8_to_floats(o4, f, T());
+            const uint4 n = ld_shared_v4(src + 16);
+            s[4] = n.x; s[5] = n.y; s[6] = n.z; s[7] = n.w;
+            q8_pick<sizeof(T) == 4>(s, uint32_t(reinterpret_cast<uintptr_t>(mat + row * ld)) & 15u, o4);
         } else {
-            q8_to_floats(s, f, T());
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o4[i] = s[i];
         }
+        q8_unit(o4, f, T());
     };
 
     uint64_t ahead = first;                                           // the next row to ask for
@@ -398,54 +379,69 @@ row_q8_ring_kernel(const RowQ8Params p) {
         if (++put == p.depth) put = 0;
     }
     for (uint64_t row = first; row < p.rows; row += step, odd ^= 1u) {
+        if constexpr (SHIFT) __syncwarp();                            // the neighbours have read the slot that is filled now
         request_row(put, ahead);
         ahead += step;
         if (++put == p.depth) put = 0;
         q8_async_wait(p.depth - 1);
+        if constexpr (SHIFT) __syncwarp();                            // the neighbours' copies have landed, too
         T* const sum = RES && p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.lds : nullptr;
         uint8_t* const q = p.q + row * p.ldq;
-        float v[NCH][8];
+        float v[NC][E];
         float ss = 0.f, big = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const uint32_t col = (c * tpr + tid) * 8;
-            const bool any = col < p.cols, all = col + 8 <= p.cols;
+        for (int c = 0; c < NC; ++c) {
+            const uint32_t col = (c * tpr + tid) * E;
+            const bool all = col + E <= p.cols;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
-            if (any) take(get, c, static_cast<const T*>(p.x), p.ldx, row, 0, v[c]);
+            for (int i = 0; i < E; ++i) v[c][i] = 0.f;
+            if (col < p.cols) {
+                take(get, c, static_cast<const T*>(p.x), p.ldx, row, 0, v[c]);
+                if constexpr (RES) {
+                    float a[E];
+                    take(get, c, static_cast<const T*>(p.r), p.ldr, row, 1, a);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) v[c][i] += a[i];
+                }
+                if (!all) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (col + i >= p.cols) v[c][i] = 0.f;
+                }
+            }
             if constexpr (RES) {
-                float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (any) take(get, c, static_cast<const T*>(p.r), p.ldr, row, UL, a);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] += a[i];
                 if (sum != nullptr) {
-                    if (SHIFT && (c * tpr + (tid | 31u)) * 8 + 8 <= p.cols) {          // the whole warp has whole pieces
-                        q8_store8_shift(sum + col, v[c], lane);
+                    if (SHIFT && (c * tpr + (tid | 31u) + 1) * E <= p.cols) {          // the whole warp has whole units
+                        q8_store_shift<T, E>(sum + col, v[c], lane);
                     } else if (!SHIFT && all) {
-                        q8_store8(sum + col, v[c]);
+                        uint32_t o[4];
+                        q8_words(v[c], o);
+                        *reinterpret_cast<uint4*>(sum + col) = make_uint4(o[0], o[1], o[2], o[3]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
+                        for (int i = 0; i < E; ++i)
                             if (col + i < p.cols) q8_store(sum + col + i, v[c][i]);
                     }
                 }
             }
             if constexpr (NORM) {
-                float a[8];
+                float a[E];
                 if (all) {
-                    q8_load8(w + col, a);
+                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(w + col));
+                    const uint32_t u4[4] = {u.x, u.y, u.z, u.w};
+                    q8_unit(u4, a, T());
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) a[i] = col + i < p.cols ? q8_load(w + col + i) : 0.f;
+                    for (int i = 0; i < E; ++i) a[i] = col + i < p.cols ? q8_load(w + col + i) : 0.f;
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < E; ++i) {
                     ss = fmaf(v[c][i], v[c][i], ss);
                     v[c][i] *= a[i];
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(big) : "f"(fabsf(v[c][i])));
+            for (int i = 0; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(big) : "f"(fabsf(v[c][i])));
         }
         if (++get == p.depth) get = 0;
         // ---- the row's sum of squares and largest magnitude (two sets of slots: one barrier a row)
@@ -456,7 +452,6 @@ row_q8_ring_kernel(const RowQ8Params p) {
         }
         top = __reduce_max_sync(0xffffffffu, top);
         if constexpr (!WARP) {
-            const uint32_t wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
             if (lane == 0) {
                 red_ss[odd][wid] = ss;
                 red_top[odd][wid] = top;
@@ -475,22 +470,24 @@ row_q8_ring_kernel(const RowQ8Params p) {
         if (tid == 0) p.scales[row] = scale;
         if (pre != 1.f) {
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] *= pre;
+                for (int i = 0; i < E; ++i) v[c][i] *= pre;
         }
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const uint32_t col = (c * tpr + tid) * 8;
-            uint2 o;
-            o.x = e4m3x2(v[c][0] * mul, v[c][1] * mul) | (e4m3x2(v[c][2] * mul, v[c][3] * mul) << 16);
-            o.y = e4m3x2(v[c][4] * mul, v[c][5] * mul) | (e4m3x2(v[c][6] * mul, v[c][7] * mul) << 16);
-            if (col + 8 <= p.cols) {
-                *reinterpret_cast<uint2*>(q + col) = o;
+        for (int c = 0; c < NC; ++c) {
+            const uint32_t col = (c * tpr + tid) * E;
+            uint32_t o[E / 4];
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i)
+                o[i] = e4m3x2(v[c][4 * i] * mul, v[c][4 * i + 1] * mul) | (e4m3x2(v[c][4 * i + 2] * mul, v[c][4 * i + 3] * mul) << 16);
+            if (col + E <= p.cols) {
+                if constexpr (E == 8) *reinterpret_cast<uint2*>(q + col) = make_uint2(o[0], o[1]);
+                else *reinterpret_cast<uint32_t*>(q + col) = o[0];
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (col + i < p.cols) q[col + i] = uint8_t((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
+                for (int i = 0; i < E; ++i)
+                    if (col + i < p.cols) q[col + i] = uint8_t(o[i / 4] >> (8 * (i & 3)));
             }
         }
     }
