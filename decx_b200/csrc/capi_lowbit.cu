@@ -111,7 +111,7 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     const bool out8 = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 && aligned16(p.w);
     // two slots of the ring have to fit: the limit is 1024 threads times two pieces of 8, or shared memory
     const uint64_t slot = uint64_t(p.cols + 511) / 512 * (rows16 ? 512 : 528) * e * (p.r != nullptr ? 2 : 1);
-    const bool ring = out8 && p.cols <= 16384 && 2 * slot <= 200 * 1024 && (p.rows > 296 || !rows16);
+    const bool ring = out8 && p.cols >= 16 && p.cols <= 16384 && 2 * slot <= 200 * 1024 && (p.rows > 296 || !rows16);
     if (!ring) return rows16 && out8 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
     if constexpr (NORM) {
         if (p.r != nullptr)

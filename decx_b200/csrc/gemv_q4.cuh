@@ -14,8 +14,8 @@
 // the arithmetic.
 //
 // Exactness and cost.  A nibble q left in the low bits of an fp16 number IS the subnormal q * 2^-24 (16 q * 2^-24 for the
-// upper nibble of a byte), and the tensor path multiplies subnormals exactly: one mask per pair of weights is all the
-// unpacking there is.  Products of lower and of upper nibbles go to accumulators of their own, and the zero point
+// upper nibble of a byte), and the tensor path multiplies subnormals exactly: a mask, or the difference of two such numbers
+// (exact as well, and not on the integer pipe, which is what limits the unpacking), is all there is per pair of weights.  Products of lower and of upper nibbles go to accumulators of their own, and the zero point
 // leaves the sum: sum (q - z) x = sum q x - z sum x, with the group sums of x computed once.  x is fp16 or e4m3, which
 // fp16 holds exactly.  All sums are fp32; the group's scale multiplies in fp32; 2^24 comes back at the end; the only
 // other rounding is the one to an fp16 result.
@@ -56,9 +56,10 @@ struct Q4Cfg {
     static constexpr int MAX_TILES = NT == 1 ? 4 : 2;
     static constexpr int RS = 16 * MAX_TILES + 4;             // floats between vectors: no bank twice
     static constexpr int WARPS = 16;                          // most per CTA
+    static constexpr uint32_t JOIN = 2048;                    // sums a CTA collects before its cluster joins them
     static constexpr uint32_t PART = 8 * NT * RS * 4;         // bytes of one warp's partial sums
-    static constexpr uint32_t SUMS = 8 * NT * 16 * MAX_TILES * 4;
-    static constexpr uint32_t smem(uint32_t warps) { return warps * (STAGES * TILE + 2 * PART) + 2 * SUMS; }
+    static constexpr uint32_t smem(uint32_t warps) { return warps * (STAGES * TILE + 2 * PART) + 2 * JOIN * 4; }
+    static_assert(8 * NT * 16 * MAX_TILES <= JOIN, "at least one block");
 };
 static_assert(Q4Cfg<1>::smem(16) <= 227 * 1024 && Q4Cfg<2>::smem(16) <= 227 * 1024, "one CTA's shared memory");
 
@@ -86,6 +87,15 @@ __device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ float half_bits(uint32_t u) { return __half2float(__ushort_as_half(uint16_t(u))); }
+
+// A word of eight nibbles as fp16 subnormals: q * 2^-24 of weights (0,4) and (2,6), 16 q * 2^-24 of (1,5) and (3,7).
+__device__ __forceinline__ void q4_pairs(uint32_t w, uint32_t (&o)[4]) {
+    const uint32_t odd = __byte_perm(w, 0, 0x4341);           // bytes 1 and 3: lower nibble + 16 * upper nibble
+    o[0] = w & 0x000f000fu;
+    o[1] = w & 0x00f000f0u;
+    o[2] = odd & 0x000f000fu;
+    o[3] = h2_bits(__hsub2(bits_h2(odd), bits_h2(o[2])));
+}
 
 // W words (1, 2 or 4) from shared memory
 template <int W>
@@ -181,62 +191,88 @@ gemv_q4_kernel(const GemvQ4Params p) {
 
     // ---- the stream of tiles: blocks, passes over K within a block, tiles within a pass
     const uint32_t my_blocks = blocks > cluster_id ? (blocks - cluster_id - 1) / clusters + 1 : 0u;
-    const uint32_t n_tiles = my_blocks * p.passes * p.tiles;
     const uint32_t lrow = lane / UNITS, lunit = lane % UNITS; // this lane's first unit of a tile; the others 32 / UNITS rows on
-    uint32_t rq_i = 0, rq_tile = 0, rq_pass = 0, rq_block = cluster_id, rq_stage = 0;
-    auto request = [&]() {
-        const uint32_t piece = piece0 + rq_pass * pass_step;
-        if (rq_i < n_tiles && piece < pieces) {
-            const uint32_t row0 = rq_block * R + rq_tile * 16 + lrow, byte = piece * (KW / 2) + lunit * 16;
-            const uint32_t n = byte < row_bytes ? min(16u, row_bytes - byte) : 0u;
-            const uint8_t* src = p.W + uint64_t(row0) * p.ldw + byte;
-            const uint32_t dst = ring + rq_stage * Cfg::TILE + lrow * PITCH;
+    constexpr uint32_t ROWS = 32 / UNITS, COPIES = 16 / ROWS; // rows per instruction, instructions per tile
+    uint32_t rq_left = my_blocks * p.passes * p.tiles, rq_tile = 0, rq_pass = 0, rq_row0 = cluster_id * R, rq_stage = ring;
+    const uint8_t* rq_src = nullptr;
+    uint32_t rq_bytes = 0;
+    const uint64_t copy_step = ROWS * p.ldw;
+    uint32_t rq_dst[2];                                       // rows that many apart have one of two swizzles
 #pragma unroll
-            for (uint32_t i = 0; i < 16u * UNITS / 32; ++i) {
-                constexpr uint32_t ROWS = 32 / UNITS;         // rows per instruction
-                const bool in = n != 0 && row0 + i * ROWS < p.rows;
-                cp_async16(dst + i * ROWS * PITCH + ((lunit ^ q4_swizzle<UNITS>(lrow + i * ROWS)) * 16), in ? src : p.W, in ? n : 0u);
-                src += ROWS * p.ldw;
+    for (uint32_t i = 0; i < 2; ++i) rq_dst[i] = (lrow + i * ROWS) * PITCH + ((lunit ^ q4_swizzle<UNITS>(lrow + i * ROWS)) * 16);
+    static_assert(2 * ROWS == 8 || (UNITS == 4 && ROWS == 8), "two swizzles cover all rows");
+    auto request_block = [&]() {                              // where this lane's share of a block's weights starts
+        const uint32_t byte = (piece0 + rq_pass * pass_step) * (KW / 2) + lunit * 16;
+        rq_bytes = byte < row_bytes ? min(16u, row_bytes - byte) : 0u;
+        rq_src = p.W + uint64_t(rq_row0 + lrow) * p.ldw + (rq_bytes ? byte : 0u);
+    };
+    request_block();
+    auto request = [&]() {
+        if (rq_left != 0 && piece0 + rq_pass * pass_step < pieces) {
+            const uint32_t row0 = rq_row0 + rq_tile * 16;
+            const uint8_t* src = rq_src;
+            if (row0 + 16 <= p.rows) {
+#pragma unroll
+                for (uint32_t i = 0; i < COPIES; ++i, src += copy_step)
+                    cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, src, rq_bytes);
+            } else {                                          // rows behind the last one become zeros
+#pragma unroll
+                for (uint32_t i = 0; i < COPIES; ++i, src += copy_step) {
+                    const bool in = row0 + lrow + i * ROWS < p.rows;
+                    cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, in ? src : p.W, in ? rq_bytes : 0u);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        ++rq_i;
-        if (++rq_stage == STAGES) rq_stage = 0;
+        if (rq_left != 0) --rq_left;
+        rq_stage += Cfg::TILE;
+        if (rq_stage == ring + STAGES * Cfg::TILE) rq_stage = ring;
+        rq_src += 16 * p.ldw;
         if (++rq_tile == p.tiles) {
             rq_tile = 0;
             if (++rq_pass == p.passes) {
                 rq_pass = 0;
-                rq_block += clusters;
+                rq_row0 += clusters * R;
             }
+            request_block();
         }
     };
     for (int d = 0; d < STAGES - 1; ++d) request();
 
     // ---- scales and zero points of rows g and g + 8 of a tile, asked for one tile ahead
     uint32_t sraw[2][(2 * GC + 3) / 4], zraw[2][(GC + 3) / 4];
-    uint32_t sq_tile = 0, sq_pass = 0, sq_block = cluster_id, sq_i = 0;
-    auto request_scales = [&]() {
+    uint32_t sq_left = my_blocks * p.passes * p.tiles, sq_tile = 0, sq_pass = 0, sq_row0 = cluster_id * R;
+    const __half* sq_s = nullptr;
+    const uint8_t* sq_z = nullptr;
+    auto scales_block = [&]() {
         const uint32_t g0 = (piece0 + sq_pass * pass_step) * GC;
-        if (sq_i < n_tiles && g0 < groups) {
+        sq_s = p.scales + uint64_t(sq_row0 + g) * p.lds + g0;
+        if constexpr (ZEROS) sq_z = p.zeros + uint64_t(sq_row0 + g) * p.ldz + g0;
+    };
+    scales_block();
+    auto request_scales = [&]() {
+        const uint32_t g0 = (piece0 + sq_pass * pass_step) * GC, row0 = sq_row0 + sq_tile * 16;
+        if (sq_left != 0 && g0 < groups) {
+            if (p.vec_s && (!ZEROS || p.vec_z) && g0 + GC <= groups && row0 + 16 <= p.rows) {
+                q4_load_bytes<2 * GC>(sq_s, sraw[0]);
+                q4_load_bytes<2 * GC>(sq_s + 8 * p.lds, sraw[1]);
+                if constexpr (ZEROS) {
+                    q4_load_bytes<GC>(sq_z, zraw[0]);
+                    q4_load_bytes<GC>(sq_z + 8 * p.ldz, zraw[1]);
+                }
+            } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // rows behind the last one repeat it: their sums are never stored
-                const uint64_t row = min(sq_block * R + sq_tile * 16 + h * 8 + g, p.rows - 1);
-                const __half* sp = p.scales + row * p.lds + g0;
-                if (p.vec_s && g0 + GC <= groups) {
-                    q4_load_bytes<2 * GC>(sp, sraw[h]);
-                } else {
+                for (int h = 0; h < 2; ++h) {
+                    // rows behind the last one repeat it: their sums are never stored
+                    const uint64_t row = min(row0 + h * 8 + g, p.rows - 1);
+                    const __half* sp = p.scales + row * p.lds + g0;
 #pragma unroll
                     for (int j = 0; j < GC; ++j) {
                         const uint32_t b = g0 + j < groups ? __half_as_ushort(sp[j]) : 0u;
                         sraw[h][j / 2] = (j & 1) ? (sraw[h][j / 2] | (b << 16)) : b;
                     }
-                }
-                if constexpr (ZEROS) {
-                    const uint8_t* zp = p.zeros + row * p.ldz + g0;
-                    if (p.vec_z && g0 + GC <= groups) {
-                        q4_load_bytes<GC>(zp, zraw[h]);
-                    } else {
+                    if constexpr (ZEROS) {
+                        const uint8_t* zp = p.zeros + row * p.ldz + g0;
 #pragma unroll
                         for (int j = 0; j < GC; ++j) {
                             const uint32_t b = g0 + j < groups ? zp[j] : 0u;
@@ -246,13 +282,16 @@ gemv_q4_kernel(const GemvQ4Params p) {
                 }
             }
         }
-        ++sq_i;
+        if (sq_left != 0) --sq_left;
+        sq_s += 16 * p.lds;
+        if constexpr (ZEROS) sq_z += 16 * p.ldz;
         if (++sq_tile == p.tiles) {
             sq_tile = 0;
             if (++sq_pass == p.passes) {
                 sq_pass = 0;
-                sq_block += clusters;
+                sq_row0 += clusters * R;
             }
+            scales_block();
         }
     };
 #pragma unroll
@@ -302,22 +341,25 @@ gemv_q4_kernel(const GemvQ4Params p) {
             static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row] = q4_out<OUT>(s);
         }
     };
-    auto join_cluster = [&](uint32_t block, uint32_t buf) {   // all CTAs' sums of a block: requested together, added in order
+    // A cluster joins several blocks at a time: its barrier has to wait for a CTA's outstanding memory accesses.
+    const uint32_t per_join = Cfg::JOIN / (R * p.n_vec);
+    auto join_cluster = [&](uint32_t b0, uint32_t n) {        // n of this cluster's blocks from b0 on, in rank order
         namespace cg = cooperative_groups;
         const cg::cluster_group cluster = cg::this_cluster();
-        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < R * p.n_vec; i += ranks * blockDim.x) {
-            float d[8];
+        float* const from = sums + ((b0 / per_join) & 1u) * Cfg::JOIN;
+        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < n * R * p.n_vec; i += ranks * blockDim.x) {
+            float d[8];                                       // requested together
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c)
-                d[c] = c < ranks ? *cluster.map_shared_rank(sums + buf * (Cfg::SUMS / 4) + i, c) : 0.f;
+            for (uint32_t c = 0; c < 8; ++c) d[c] = c < ranks ? *cluster.map_shared_rank(from + i, c) : 0.f;
             float s = 0.f;
 #pragma unroll
             for (uint32_t c = 0; c < 8; ++c) s += d[c];
-            store(block, i, s);
+            const uint32_t k = i / (R * p.n_vec);
+            store(cluster_id + (b0 + k) * clusters, i - k * R * p.n_vec, s);
         }
     };
 
-    uint32_t stage = 0;
+    uint32_t stage = ring;
     const uint32_t sw = q4_swizzle<UNITS>(g) * 16;            // rows g and g + 8 share it
     for (uint32_t b = 0; b < my_blocks; ++b) {
         const uint32_t block = cluster_id + b * clusters, buf = b & 1u;
@@ -347,7 +389,7 @@ gemv_q4_kernel(const GemvQ4Params p) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
                 if (piece < pieces) {
-                    const uint32_t wrow = ring + stage * Cfg::TILE + g * PITCH;
+                    const uint32_t wrow = stage + g * PITCH;
 #pragma unroll
                     for (int gi = 0; gi < GC; ++gi) {
                         uint32_t wa[WPL], wb[WPL];            // rows g and g + 8
@@ -356,17 +398,18 @@ gemv_q4_kernel(const GemvQ4Params p) {
                         float lo[NT][4], hi[NT][4];
 #pragma unroll
                         for (int j = 0; j < WPL; ++j) {
-                            constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
-                            const uint32_t wa8 = wa[j] >> 8, wb8 = wb[j] >> 8;
+                            uint32_t a[4], c[4];              // pairs (0,4) (1,5) (2,6) (3,7) of rows g and g + 8
+                            q4_pairs(wa[j], a);
+                            q4_pairs(wb[j], c);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 const uint4 x = xr[gi * WPL + j][n];
                                 if (j == 0) {
-                                    mma_16816_first(lo[n], wa[j] & L, wb[j] & L, wa8 & L, wb8 & L, x.x, x.y);
-                                    mma_16816_first(hi[n], wa[j] & H, wb[j] & H, wa8 & H, wb8 & H, x.z, x.w);
+                                    mma_16816_first(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
+                                    mma_16816_first(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
                                 } else {
-                                    mma_16816(lo[n], wa[j] & L, wb[j] & L, wa8 & L, wb8 & L, x.x, x.y);
-                                    mma_16816(hi[n], wa[j] & H, wb[j] & H, wa8 & H, wb8 & H, x.z, x.w);
+                                    mma_16816(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
+                                    mma_16816(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
                                 }
                             }
                         }
@@ -380,7 +423,8 @@ gemv_q4_kernel(const GemvQ4Params p) {
                             }
                     }
                 }
-                if (++stage == STAGES) stage = 0;
+                stage += Cfg::TILE;
+                if (stage == ring + STAGES * Cfg::TILE) stage = ring;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -393,23 +437,27 @@ gemv_q4_kernel(const GemvQ4Params p) {
         }
         // ---- join.  Two sets of partial sums: what the next block writes is not what this one reads.
         __syncthreads();
-        if (ranks > 1 && b > 0) {
+        const uint32_t in_join = b % per_join;
+        if (ranks > 1 && in_join == 0 && b > 0) {             // before its half of `sums` is written again
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-            join_cluster(block - clusters, buf ^ 1u);
+            join_cluster(b - per_join, per_join);
         }
+        float* const own = sums + ((b / per_join) & 1u) * Cfg::JOIN + in_join * R * p.n_vec;
         for (uint32_t i = threadIdx.x; i < R * p.n_vec; i += blockDim.x) {
             const float* at = parts + buf * warps * (Cfg::PART / 4) + i / R * RS + i % R;
             float s = 0.f;
             for (uint32_t w = 0; w < active; ++w) s += at[w * (Cfg::PART / 4)];
-            if (ranks > 1) sums[buf * (Cfg::SUMS / 4) + i] = s;
+            if (ranks > 1) own[i] = s;
             else store(block, i, s);
         }
-        if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (ranks > 1 && (in_join + 1 == per_join || b + 1 == my_blocks))
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
     if (ranks > 1) {
         if (my_blocks > 0) {
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-            join_cluster(cluster_id + (my_blocks - 1) * clusters, (my_blocks - 1) & 1u);
+            const uint32_t b0 = (my_blocks - 1) / per_join * per_join;
+            join_cluster(b0, my_blocks - b0);
         }
         cluster_sync_all();                                   // nobody leaves while its sums are being read
     }

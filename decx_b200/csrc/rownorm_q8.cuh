@@ -303,6 +303,11 @@ __device__ __forceinline__ void q8_store_shift(T* at, const float (&f)[E], uint3
         if ((lane == 0 && i < head) || (lane == 31 && i >= head)) q8_store(at + i, f[i]);
 }
 
+// the larger of big, |a| and |b|; NaN if one of them is
+__device__ __forceinline__ void q8_max3(float& big, float a, float b) {
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(big) : "f"(a), "f"(b));
+}
+
 template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
 __global__ void __launch_bounds__(WARP ? 256 : 1024)
 row_q8_ring_kernel(const RowQ8Params p) {
@@ -316,55 +321,78 @@ row_q8_ring_kernel(const RowQ8Params p) {
     const uint32_t step = WARP ? gridDim.x * warps : gridDim.x;
     const uint32_t first = WARP ? blockIdx.x * warps + wid : blockIdx.x;
     constexpr uint32_t WARP_BYTES = (SHIFT ? 33 : 32) * 16;           // of one warp's units
+    const uint32_t unit_bytes = warps * WARP_BYTES, slot_bytes = unit_bytes * NC * MATS;
     const uint32_t mine = smem_u32(q8_ring) + wid * WARP_BYTES + lane * 16;
-    const T* const w = static_cast<const T*>(p.w);
+    const int32_t row_bytes = int32_t(p.cols * sizeof(T));
 
-    auto slot_at = [&](uint32_t slot, int c, int m) { return mine + ((slot * NC + c) * MATS + m) * warps * WARP_BYTES; };
-    // ask for this thread's units of a row
-    auto request = [&](uint32_t slot, const T* mat, uint64_t ld, uint64_t row, int m) {
-        const T* const rp = mat + row * ld;
-        const uint8_t* const end = reinterpret_cast<const uint8_t*>(rp + p.cols);
-        const uint8_t* const begin = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(rp) & ~uintptr_t(15));
+    // what stays the same for every row: the thread's first bytes, and its pieces of the weight
+    uint32_t w[NORM ? NC : 1][4];
+    if constexpr (NORM) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint8_t* at = begin + uint64_t(c * tpr + tid) * 16;
-            const uint32_t dst = slot_at(slot, c, m);
+            const uint32_t col = (c * tpr + tid) * E;
+            const T* wp = static_cast<const T*>(p.w) + col;
+            if (col + E <= p.cols) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wp));
+                w[c][0] = u.x; w[c][1] = u.y; w[c][2] = u.z; w[c][3] = u.w;
+            } else {
+                float a[E];
 #pragma unroll
-            for (int extra = 0; extra < (SHIFT ? 2 : 1); ++extra) {
-                if (extra == 1) {
-                    if (lane != 31) break;                            // the unit behind the warp's last one
-                    at += 16;
-                }
-                if (at >= end) break;
-                const int64_t left = end - at;
-                if (SHIFT && at < reinterpret_cast<const uint8_t*>(mat)) {
-                    // the matrix itself starts inside this unit: element by element
-                    const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(rp)) & 15u;
-                    T* const own = reinterpret_cast<T*>(q8_ring + (dst - smem_u32(q8_ring)) + o);
-                    for (uint32_t i = 0; i * sizeof(T) + o < 16 && i < p.cols; ++i) own[i] = rp[i];
-                } else {
-                    q8_async16(dst + extra * 16, at, left >= 16 ? 16u : uint32_t(left));
-                }
+                for (int i = 0; i < E; ++i) a[i] = col + i < p.cols ? q8_load(wp + i) : 0.f;
+                q8_words(a, w[c]);
             }
         }
+    }
+
+    // ask for this thread's units of a row
+    const uint8_t* next_x = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.x) + uint64_t(first) * p.ldx);
+    const uint8_t* next_r = RES ? reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.r) + uint64_t(first) * p.ldr) : nullptr;
+    auto request = [&](uint32_t dst, const uint8_t* rp, const void* mat) {
+        const uint32_t o = SHIFT ? uint32_t(reinterpret_cast<uintptr_t>(rp)) & 15u : 0u;
+        const uint8_t* const begin = rp - o;
+        if (SHIFT && rp == mat && o != 0) {
+            // the matrix itself starts inside its first unit: that one element by element
+            if (tid == 0) {
+                const T* from = reinterpret_cast<const T*>(rp);
+                T* const own = reinterpret_cast<T*>(q8_ring + (dst - smem_u32(q8_ring)) + o);
+                for (uint32_t i = 0; i * sizeof(T) + o < 16 && i < p.cols; ++i) own[i] = from[i];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const uint32_t off = (c * tpr + tid) * 16;
+            const int32_t left = row_bytes + int32_t(o) - int32_t(off);
+            if (left > 0 && !(SHIFT && off == 0 && rp == mat && o != 0))
+                q8_async16(dst + c * unit_bytes, begin + off, left >= 16 ? 16u : uint32_t(left));
+            if (SHIFT && lane == 31 && left > 16)                     // the unit behind the warp's last one
+                q8_async16(dst + c * unit_bytes + 16, begin + off + 16, left >= 32 ? 16u : uint32_t(left - 16));
+        }
     };
-    auto request_row = [&](uint32_t slot, uint64_t row) {
-        if (row < p.rows) {
-            request(slot, static_cast<const T*>(p.x), p.ldx, row, 0);
-            if constexpr (RES) request(slot, static_cast<const T*>(p.r), p.ldr, row, 1);
+    uint64_t ahead = first;                                           // the next row to ask for
+    uint32_t put = 0, get = 0, odd = 0;                               // byte offsets of slots
+    auto request_row = [&]() {
+        if (ahead < p.rows) {
+            request(mine + put, next_x, p.x);
+            next_x += uint64_t(step) * p.ldx * sizeof(T);
+            if constexpr (RES) {
+                request(mine + put + NC * unit_bytes, next_r, p.r);
+                next_r += uint64_t(step) * p.ldr * sizeof(T);
+            }
         }
         q8_async_commit();
+        ahead += step;
+        put += slot_bytes;
+        if (put == p.depth * slot_bytes) put = 0;
     };
     // this thread's elements of a unit; what lies behind the row's end is not zero
-    auto take = [&](uint32_t slot, int c, const T* mat, uint64_t ld, uint64_t row, int m, float (&f)[E]) {
-        const uint32_t src = slot_at(slot, c, m);
+    auto take = [&](uint32_t src, uint32_t o, float (&f)[E]) {
         uint32_t s[8], o4[4];
         const uint4 v = ld_shared_v4(src);
         s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
         if constexpr (SHIFT) {
             const uint4 n = ld_shared_v4(src + 16);
             s[4] = n.x; s[5] = n.y; s[6] = n.z; s[7] = n.w;
-            q8_pick<sizeof(T) == 4>(s, uint32_t(reinterpret_cast<uintptr_t>(mat + row * ld)) & 15u, o4);
+            q8_pick<sizeof(T) == 4>(s, o, o4);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o4[i] = s[i];
@@ -372,42 +400,34 @@ row_q8_ring_kernel(const RowQ8Params p) {
         q8_unit(o4, f, T());
     };
 
-    uint64_t ahead = first;                                           // the next row to ask for
-    uint32_t put = 0, get = 0, odd = 0;
-    for (uint32_t d = 0; d + 1 < p.depth; ++d, ahead += step) {
-        request_row(put, ahead);
-        if (++put == p.depth) put = 0;
-    }
+    for (uint32_t d = 0; d + 1 < p.depth; ++d) request_row();
+    const uint64_t lx = p.ldx * sizeof(T), lr = p.ldr * sizeof(T);
+    T* sum = RES && p.sum != nullptr ? static_cast<T*>(p.sum) + uint64_t(first) * p.lds : nullptr;
+    uint8_t* q = p.q + uint64_t(first) * p.ldq;
     for (uint64_t row = first; row < p.rows; row += step, odd ^= 1u) {
         if constexpr (SHIFT) __syncwarp();                            // the neighbours have read the slot that is filled now
-        request_row(put, ahead);
-        ahead += step;
-        if (++put == p.depth) put = 0;
+        request_row();
         q8_async_wait(p.depth - 1);
         if constexpr (SHIFT) __syncwarp();                            // the neighbours' copies have landed, too
-        T* const sum = RES && p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.lds : nullptr;
-        uint8_t* const q = p.q + row * p.ldq;
+        const uint32_t ox = SHIFT ? uint32_t(reinterpret_cast<uintptr_t>(p.x) + row * lx) & 15u : 0u;
+        const uint32_t orr = SHIFT && RES ? uint32_t(reinterpret_cast<uintptr_t>(p.r) + row * lr) & 15u : 0u;
         float v[NC][E];
         float ss = 0.f, big = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const uint32_t col = (c * tpr + tid) * E;
             const bool all = col + E <= p.cols;
+            take(mine + get + c * unit_bytes, ox, v[c]);
+            if constexpr (RES) {
+                float a[E];
+                take(mine + get + (NC + c) * unit_bytes, orr, a);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[c][i] = 0.f;
-            if (col < p.cols) {
-                take(get, c, static_cast<const T*>(p.x), p.ldx, row, 0, v[c]);
-                if constexpr (RES) {
-                    float a[E];
-                    take(get, c, static_cast<const T*>(p.r), p.ldr, row, 1, a);
+                for (int i = 0; i < E; ++i) v[c][i] += a[i];
+            }
+            if (!all) {
 #pragma unroll
-                    for (int i = 0; i < E; ++i) v[c][i] += a[i];
-                }
-                if (!all) {
-#pragma unroll
-                    for (int i = 0; i < E; ++i)
-                        if (col + i >= p.cols) v[c][i] = 0.f;
-                }
+                for (int i = 0; i < E; ++i)
+                    if (col + i >= p.cols) v[c][i] = 0.f;
             }
             if constexpr (RES) {
                 if (sum != nullptr) {
@@ -426,14 +446,7 @@ row_q8_ring_kernel(const RowQ8Params p) {
             }
             if constexpr (NORM) {
                 float a[E];
-                if (all) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(w + col));
-                    const uint32_t u4[4] = {u.x, u.y, u.z, u.w};
-                    q8_unit(u4, a, T());
-                } else {
-#pragma unroll
-                    for (int i = 0; i < E; ++i) a[i] = col + i < p.cols ? q8_load(w + col + i) : 0.f;
-                }
+                q8_unit(w[c], a, T());
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     ss = fmaf(v[c][i], v[c][i], ss);
@@ -441,9 +454,10 @@ row_q8_ring_kernel(const RowQ8Params p) {
                 }
             }
 #pragma unroll
-            for (int i = 0; i < E; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(big) : "f"(fabsf(v[c][i])));
+            for (int i = 0; i < E; i += 2) q8_max3(big, v[c][i], v[c][i + 1]);
         }
-        if (++get == p.depth) get = 0;
+        get += slot_bytes;
+        if (get == p.depth * slot_bytes) get = 0;
         // ---- the row's sum of squares and largest magnitude (two sets of slots: one barrier a row)
         uint32_t top = __float_as_uint(big);
         if constexpr (NORM) {
@@ -490,6 +504,8 @@ row_q8_ring_kernel(const RowQ8Params p) {
                     if (col + i < p.cols) q[col + i] = uint8_t(o[i / 4] >> (8 * (i & 3)));
             }
         }
+        q += uint64_t(step) * p.ldq;
+        if (RES && sum != nullptr) sum += uint64_t(step) * p.lds;
     }
 }
 
