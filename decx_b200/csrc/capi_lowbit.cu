@@ -176,18 +176,9 @@ int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
         if (clusters < 1) clusters = 1;
         held[p.ranks - 1][warps - 1].store(clusters, std::memory_order_relaxed);
     }
-    // the height of the blocks that is done in the fewest turns (the larger one of equals: fewer joins)
-    uint64_t best = ~0ull;
-    for (uint32_t tiles = Cfg::MAX_TILES; tiles >= 1; tiles /= 2) {
-        const uint64_t blocks = (uint64_t(p.rows) + 16 * tiles - 1) / (16 * tiles);
-        const uint64_t turns = (blocks + clusters - 1) / clusters * tiles;
-        if (turns < best) {
-            best = turns;
-            p.tiles = tiles;
-        }
-    }
-    const uint64_t blocks = (uint64_t(p.rows) + 16 * p.tiles - 1) / (16 * p.tiles);
-    const uint64_t n = blocks < uint64_t(clusters) ? blocks : uint64_t(clusters);
+    const uint64_t tiles = (uint64_t(p.rows) + Cfg::TR - 1) / Cfg::TR;
+    p.tiles = uint32_t((tiles + clusters - 1) / clusters);
+    const uint64_t n = (tiles + p.tiles - 1) / p.tiles;
     return launch_cluster(kern, unsigned(n * p.ranks), 32 * warps, Cfg::smem(warps), p.ranks, s, p);
 }
 

@@ -43,7 +43,7 @@ struct GemvQ4Params {
     uint32_t rows, cols, n_vec;
     uint32_t ranks;            // CTAs that share a block of rows = cluster size, at most 8
     uint32_t passes;           // 1 unless K is longer than ranks * warps pieces
-    uint32_t tiles;            // 16-row tiles per block of rows: 1, 2 or 4
+    uint32_t tiles;            // tiles of a cluster: its share of the rows
     int vec_s, vec_z;          // a tile's scales / zero points of one row may be read at once
 };
 
@@ -51,15 +51,18 @@ template <int NT>
 struct Q4Cfg {
     static constexpr int KW = NT == 1 ? 256 : 128;            // columns of a warp
     static constexpr int UNITS = KW / 32;                     // 16-byte units of a row of a tile
-    static constexpr uint32_t TILE = 16 * UNITS * 16;         // bytes
-    static constexpr int STAGES = NT == 1 ? 4 : 8;            // 8 KB per warp
-    static constexpr int MAX_TILES = NT == 1 ? 4 : 2;
-    static constexpr int RS = 16 * MAX_TILES + 4;             // floats between vectors: no bank twice
+    static constexpr int SUB = NT;                            // 16-row parts of a tile
+    static constexpr int TR = 16 * SUB;                       // rows of a tile
+    static constexpr uint32_t TILE = TR * UNITS * 16;         // bytes: 2 KB
+    static constexpr int STAGES = 4;
+    static constexpr int BLOCK = NT == 1 ? 4 : 1;             // tiles between two joins of the CTA's warps
+    static constexpr int R = TR * BLOCK;
+    static constexpr int RS = R + 4;                          // floats between vectors: no bank twice
     static constexpr int WARPS = 16;                          // most per CTA
     static constexpr uint32_t JOIN = 2048;                    // sums a CTA collects before its cluster joins them
     static constexpr uint32_t PART = 8 * NT * RS * 4;         // bytes of one warp's partial sums
     static constexpr uint32_t smem(uint32_t warps) { return warps * (STAGES * TILE + 2 * PART) + 2 * JOIN * 4; }
-    static_assert(8 * NT * 16 * MAX_TILES <= JOIN, "at least one block");
+    static_assert(8 * NT * R <= JOIN, "at least one block");
 };
 static_assert(Q4Cfg<1>::smem(16) <= 227 * 1024 && Q4Cfg<2>::smem(16) <= 227 * 1024, "one CTA's shared memory");
 
@@ -165,142 +168,134 @@ __device__ __forceinline__ void q4_load_x(const GemvQ4Params& p, uint32_t v, uin
     }
 }
 
-// NT: tiles of eight vectors (1 or 2).  X8: x is e4m3.  grid = clusters x ranks, ranks innermost; a cluster takes every
-// (gridDim.x / ranks)-th block of rows.
+// NT: tiles of eight vectors (1 or 2).  X8: x is e4m3.  grid = clusters x ranks, ranks innermost; a cluster takes
+// p.tiles neighbouring tiles of rows.
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
 __global__ void __launch_bounds__(32 * Q4Cfg<NT>::WARPS, 1)
 gemv_q4_kernel(const GemvQ4Params p) {
     using Cfg = Q4Cfg<NT>;
-    constexpr int KW = Cfg::KW, UNITS = Cfg::UNITS, STAGES = Cfg::STAGES, RS = Cfg::RS;
+    constexpr int KW = Cfg::KW, UNITS = Cfg::UNITS, STAGES = Cfg::STAGES, RS = Cfg::RS, SUB = Cfg::SUB, TR = Cfg::TR;
     constexpr int WPL = GROUP / 32;                           // words a lane holds of a row's group
     constexpr int GC = KW / GROUP;                            // groups of a warp's piece
     constexpr uint32_t PITCH = UNITS * 16;
     extern __shared__ __align__(128) uint8_t q4_smem[];      // the swizzle works on address bits 4 to 6
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t warps = blockDim.x >> 5, ranks = p.ranks, rank = blockIdx.x % ranks;
-    const uint32_t cluster_id = blockIdx.x / ranks, clusters = gridDim.x / ranks;
-    const uint32_t R = 16 * p.tiles, blocks = (p.rows + R - 1) / R;
+    const uint32_t tile0 = blockIdx.x / ranks * p.tiles;      // the cluster's rows: [row0, row0 + n_tiles * TR)
+    const uint32_t row0 = tile0 * TR, all_tiles = (p.rows + TR - 1) / TR;
+    const uint32_t n_tiles = min(p.tiles, all_tiles - tile0);
     const uint32_t row_bytes = (p.cols + 1) / 2, groups = (p.cols + GROUP - 1) / GROUP;
     const uint32_t pieces = (p.cols + KW - 1) / KW;
     const uint32_t ring = smem_u32(q4_smem) + warp * STAGES * Cfg::TILE;
     float* const parts = reinterpret_cast<float*>(q4_smem + warps * STAGES * Cfg::TILE);      // [2][warp][vector][RS]
-    float* const sums = parts + 2 * warps * (Cfg::PART / 4);                                  // [2][vector][R]
+    float* const sums = parts + 2 * warps * (Cfg::PART / 4);                                  // [2][block][vector][R]
     // pieces this CTA covers in pass 0 (later passes have at most as many: their missing warps add nothing)
     const uint32_t piece0 = rank * warps + warp, pass_step = ranks * warps;
     const uint32_t active = min(warps, pieces > rank * warps ? pieces - rank * warps : 0u);
 
-    // ---- the stream of tiles: blocks, passes over K within a block, tiles within a pass
-    const uint32_t my_blocks = blocks > cluster_id ? (blocks - cluster_id - 1) / clusters + 1 : 0u;
+    // ---- the stream of tiles: down the rows; with several passes over K, pass by pass within a block of BLOCK tiles
+    struct Place {                                            // where a stream is
+        uint32_t row, left, tile, pass;
+    };
+    // moves a stream on; true: to another place than the next tile down
+    auto advance = [&](Place& s) {
+        s.row += TR;
+        --s.left;
+        if (p.passes == 1) return false;
+        const uint32_t in_block = min(uint32_t(Cfg::BLOCK), n_tiles - (s.row - TR * (s.tile + 1) - row0) / TR);
+        if (++s.tile < in_block) return false;
+        s.tile = 0;
+        if (++s.pass == p.passes) s.pass = 0;
+        else s.row -= TR * in_block;
+        return true;
+    };
+
     const uint32_t lrow = lane / UNITS, lunit = lane % UNITS; // this lane's first unit of a tile; the others 32 / UNITS rows on
-    constexpr uint32_t ROWS = 32 / UNITS, COPIES = 16 / ROWS; // rows per instruction, instructions per tile
-    uint32_t rq_left = my_blocks * p.passes * p.tiles, rq_tile = 0, rq_pass = 0, rq_row0 = cluster_id * R, rq_stage = ring;
-    const uint8_t* rq_src = nullptr;
-    uint32_t rq_bytes = 0;
-    const uint64_t copy_step = ROWS * p.ldw;
+    constexpr uint32_t ROWS = 32 / UNITS, COPIES = TR / ROWS; // rows per instruction, instructions per tile
     uint32_t rq_dst[2];                                       // rows that many apart have one of two swizzles
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) rq_dst[i] = (lrow + i * ROWS) * PITCH + ((lunit ^ q4_swizzle<UNITS>(lrow + i * ROWS)) * 16);
-    static_assert(2 * ROWS == 8 || (UNITS == 4 && ROWS == 8), "two swizzles cover all rows");
-    auto request_block = [&]() {                              // where this lane's share of a block's weights starts
-        const uint32_t byte = (piece0 + rq_pass * pass_step) * (KW / 2) + lunit * 16;
+    Place rq = {row0, n_tiles * p.passes, 0, 0};
+    uint32_t rq_stage = ring, rq_bytes = 0;
+    const uint8_t* rq_src = nullptr;
+    auto weights_at = [&]() {
+        const uint32_t byte = (piece0 + rq.pass * pass_step) * (KW / 2) + lunit * 16;
         rq_bytes = byte < row_bytes ? min(16u, row_bytes - byte) : 0u;
-        rq_src = p.W + uint64_t(rq_row0 + lrow) * p.ldw + (rq_bytes ? byte : 0u);
+        rq_src = p.W + uint64_t(rq.row + lrow) * p.ldw + (rq_bytes ? byte : 0u);
     };
-    request_block();
+    weights_at();
+    const uint64_t copy_step = ROWS * p.ldw;
     auto request = [&]() {
-        if (rq_left != 0 && piece0 + rq_pass * pass_step < pieces) {
-            const uint32_t row0 = rq_row0 + rq_tile * 16;
-            const uint8_t* src = rq_src;
-            if (row0 + 16 <= p.rows) {
+        if (rq.left != 0) {
+            if (piece0 + rq.pass * pass_step < pieces) {
+                const uint8_t* src = rq_src;
+                if (rq.row + TR <= p.rows) {
 #pragma unroll
-                for (uint32_t i = 0; i < COPIES; ++i, src += copy_step)
-                    cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, src, rq_bytes);
-            } else {                                          // rows behind the last one become zeros
+                    for (uint32_t i = 0; i < COPIES; ++i, src += copy_step)
+                        cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, src, rq_bytes);
+                } else {                                      // rows behind the last one become zeros
 #pragma unroll
-                for (uint32_t i = 0; i < COPIES; ++i, src += copy_step) {
-                    const bool in = row0 + lrow + i * ROWS < p.rows;
-                    cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, in ? src : p.W, in ? rq_bytes : 0u);
+                    for (uint32_t i = 0; i < COPIES; ++i, src += copy_step) {
+                        const bool in = rq.row + lrow + i * ROWS < p.rows;
+                        cp_async16(rq_stage + rq_dst[i & 1] + (i >> 1) * 2 * ROWS * PITCH, in ? src : p.W, in ? rq_bytes : 0u);
+                    }
                 }
             }
+            rq_src += TR * p.ldw;
+            if (advance(rq)) weights_at();
+            rq_stage = rq_stage + Cfg::TILE == ring + STAGES * Cfg::TILE ? ring : rq_stage + Cfg::TILE;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (rq_left != 0) --rq_left;
-        rq_stage += Cfg::TILE;
-        if (rq_stage == ring + STAGES * Cfg::TILE) rq_stage = ring;
-        rq_src += 16 * p.ldw;
-        if (++rq_tile == p.tiles) {
-            rq_tile = 0;
-            if (++rq_pass == p.passes) {
-                rq_pass = 0;
-                rq_row0 += clusters * R;
-            }
-            request_block();
-        }
     };
     for (int d = 0; d < STAGES - 1; ++d) request();
 
-    // ---- scales and zero points of rows g and g + 8 of a tile, asked for one tile ahead
-    uint32_t sraw[2][(2 * GC + 3) / 4], zraw[2][(GC + 3) / 4];
-    uint32_t sq_left = my_blocks * p.passes * p.tiles, sq_tile = 0, sq_pass = 0, sq_row0 = cluster_id * R;
+    // ---- scales and zero points of rows g, g + 8, ... of a tile, asked for one tile ahead
+    uint32_t sraw[2 * SUB][(2 * GC + 3) / 4], zraw[2 * SUB][(GC + 3) / 4];
+    Place sq = {row0, n_tiles * p.passes, 0, 0};
     const __half* sq_s = nullptr;
     const uint8_t* sq_z = nullptr;
-    auto scales_block = [&]() {
-        const uint32_t g0 = (piece0 + sq_pass * pass_step) * GC;
-        sq_s = p.scales + uint64_t(sq_row0 + g) * p.lds + g0;
-        if constexpr (ZEROS) sq_z = p.zeros + uint64_t(sq_row0 + g) * p.ldz + g0;
+    bool sq_fast = false;
+    auto scales_at = [&]() {
+        const uint32_t g0 = (piece0 + sq.pass * pass_step) * GC;
+        sq_fast = p.vec_s && (!ZEROS || p.vec_z) && g0 + GC <= groups;
+        sq_s = p.scales + uint64_t(sq.row + g) * p.lds + g0;
+        if constexpr (ZEROS) sq_z = p.zeros + uint64_t(sq.row + g) * p.ldz + g0;
     };
-    scales_block();
+    scales_at();
     auto request_scales = [&]() {
-        const uint32_t g0 = (piece0 + sq_pass * pass_step) * GC, row0 = sq_row0 + sq_tile * 16;
-        if (sq_left != 0 && g0 < groups) {
-            if (p.vec_s && (!ZEROS || p.vec_z) && g0 + GC <= groups && row0 + 16 <= p.rows) {
-                q4_load_bytes<2 * GC>(sq_s, sraw[0]);
-                q4_load_bytes<2 * GC>(sq_s + 8 * p.lds, sraw[1]);
-                if constexpr (ZEROS) {
-                    q4_load_bytes<GC>(sq_z, zraw[0]);
-                    q4_load_bytes<GC>(sq_z + 8 * p.ldz, zraw[1]);
-                }
-            } else {
+        if (sq.left == 0) return;
+        if (sq_fast && sq.row + TR <= p.rows) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // rows behind the last one repeat it: their sums are never stored
-                    const uint64_t row = min(row0 + h * 8 + g, p.rows - 1);
-                    const __half* sp = p.scales + row * p.lds + g0;
+            for (int h = 0; h < 2 * SUB; ++h) {
+                q4_load_bytes<2 * GC>(sq_s + h * 8 * p.lds, sraw[h]);
+                if constexpr (ZEROS) q4_load_bytes<GC>(sq_z + h * 8 * p.ldz, zraw[h]);
+            }
+        } else {
+            const uint32_t g0 = (piece0 + sq.pass * pass_step) * GC;
+#pragma unroll
+            for (int h = 0; h < 2 * SUB; ++h) {
+                // rows behind the last one repeat it: their sums are never stored
+                const uint64_t row = min(sq.row + h * 8 + g, p.rows - 1);
+                const __half* sp = p.scales + row * p.lds + g0;
+#pragma unroll
+                for (int j = 0; j < GC; ++j) {
+                    const uint32_t b = g0 + j < groups ? __half_as_ushort(sp[j]) : 0u;
+                    sraw[h][j / 2] = (j & 1) ? (sraw[h][j / 2] | (b << 16)) : b;
+                }
+                if constexpr (ZEROS) {
+                    const uint8_t* zp = p.zeros + row * p.ldz + g0;
 #pragma unroll
                     for (int j = 0; j < GC; ++j) {
-                        const uint32_t b = g0 + j < groups ? __half_as_ushort(sp[j]) : 0u;
-                        sraw[h][j / 2] = (j & 1) ? (sraw[h][j / 2] | (b << 16)) : b;
-                    }
-                    if constexpr (ZEROS) {
-                        const uint8_t* zp = p.zeros + row * p.ldz + g0;
-#pragma unroll
-                        for (int j = 0; j < GC; ++j) {
-                            const uint32_t b = g0 + j < groups ? zp[j] : 0u;
-                            zraw[h][j / 4] = (j & 3) ? (zraw[h][j / 4] | (b << (8 * (j & 3)))) : b;
-                        }
+                        const uint32_t b = g0 + j < groups ? zp[j] : 0u;
+                        zraw[h][j / 4] = (j & 3) ? (zraw[h][j / 4] | (b << (8 * (j & 3)))) : b;
                     }
                 }
             }
         }
-        if (sq_left != 0) --sq_left;
-        sq_s += 16 * p.lds;
-        if constexpr (ZEROS) sq_z += 16 * p.ldz;
-        if (++sq_tile == p.tiles) {
-            sq_tile = 0;
-            if (++sq_pass == p.passes) {
-                sq_pass = 0;
-                sq_row0 += clusters * R;
-            }
-            scales_block();
-        }
+        sq_s += TR * p.lds;
+        if constexpr (ZEROS) sq_z += TR * p.ldz;
+        if (advance(sq)) scales_at();
     };
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int j = 0; j < (2 * GC + 3) / 4; ++j) sraw[h][j] = 0u;
-#pragma unroll
-        for (int j = 0; j < (GC + 3) / 4; ++j) zraw[h][j] = 0u;
-    }
     request_scales();
 
     // ---- this warp's x: registers in product order, and the group sums of the vectors whose columns this lane gets
@@ -334,48 +329,49 @@ gemv_q4_kernel(const GemvQ4Params p) {
     if (p.passes == 1) load_x(piece0);
 
     auto store = [&](uint32_t block, uint32_t i, float s) {   // i = vector * R + row
-        const uint32_t v = i / R, row = block * R + i % R;
-        if (row < p.rows) {
+        const uint32_t v = i / Cfg::R, r = block * Cfg::R + i % Cfg::R, row = row0 + r;
+        if (r < n_tiles * TR && row < p.rows) {               // the last block may have fewer tiles
             s *= 0x1p24f;
             if (p.xs != nullptr) s *= __ldg(p.xs + v);
             static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row] = q4_out<OUT>(s);
         }
     };
     // A cluster joins several blocks at a time: its barrier has to wait for a CTA's outstanding memory accesses.
-    const uint32_t per_join = Cfg::JOIN / (R * p.n_vec);
+    const uint32_t block_sums = Cfg::R * p.n_vec, per_join = Cfg::JOIN / block_sums;
+    const uint32_t blocks = (n_tiles + Cfg::BLOCK - 1) / Cfg::BLOCK;
     auto join_cluster = [&](uint32_t b0, uint32_t n) {        // n of this cluster's blocks from b0 on, in rank order
         namespace cg = cooperative_groups;
         const cg::cluster_group cluster = cg::this_cluster();
         float* const from = sums + ((b0 / per_join) & 1u) * Cfg::JOIN;
-        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < n * R * p.n_vec; i += ranks * blockDim.x) {
+        for (uint32_t i = rank * blockDim.x + threadIdx.x; i < n * block_sums; i += ranks * blockDim.x) {
             float d[8];                                       // requested together
 #pragma unroll
             for (uint32_t c = 0; c < 8; ++c) d[c] = c < ranks ? *cluster.map_shared_rank(from + i, c) : 0.f;
             float s = 0.f;
 #pragma unroll
             for (uint32_t c = 0; c < 8; ++c) s += d[c];
-            const uint32_t k = i / (R * p.n_vec);
-            store(cluster_id + (b0 + k) * clusters, i - k * R * p.n_vec, s);
+            const uint32_t k = i / block_sums;
+            store(b0 + k, i - k * block_sums, s);
         }
     };
 
     uint32_t stage = ring;
-    const uint32_t sw = q4_swizzle<UNITS>(g) * 16;            // rows g and g + 8 share it
-    for (uint32_t b = 0; b < my_blocks; ++b) {
-        const uint32_t block = cluster_id + b * clusters, buf = b & 1u;
-        float* const part = parts + (buf * warps + warp) * (Cfg::PART / 4);
+    const uint32_t sw = q4_swizzle<UNITS>(g) * 16;            // rows 8 apart share it
+    for (uint32_t b = 0; b < blocks; ++b) {
+        const uint32_t buf = b & 1u, in_block = min(uint32_t(Cfg::BLOCK), n_tiles - b * Cfg::BLOCK);
+        float* const part = parts + (buf * warps + warp) * (Cfg::PART / 4) + 2 * t * RS + g;
         for (uint32_t pass = 0; pass < p.passes; ++pass) {
             const uint32_t piece = piece0 + pass * pass_step;
             if (p.passes > 1) load_x(piece);
-            for (uint32_t tile = 0; tile < p.tiles; ++tile) {
+            for (uint32_t tile = 0; tile < in_block; ++tile) {
                 // the stage that is asked for now was read in the previous turn, by all lanes
                 __syncwarp();
                 request();
                 asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
                 __syncwarp();                                 // every lane's copies of this tile have landed
-                float sc[2][GC], nz[2][GC];
+                float sc[2 * SUB][GC], nz[2 * SUB][GC];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2 * SUB; ++h)
 #pragma unroll
                     for (int j = 0; j < GC; ++j) {
                         sc[h][j] = half_bits(sraw[h][j / 2] >> (16 * (j & 1)));
@@ -383,56 +379,57 @@ gemv_q4_kernel(const GemvQ4Params p) {
                         else nz[h][j] = -8.f;
                     }
                 request_scales();
-                float acc[NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int sub = 0; sub < SUB; ++sub) {
+                    float acc[NT][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-                if (piece < pieces) {
-                    const uint32_t wrow = stage + g * PITCH;
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int gi = 0; gi < GC; ++gi) {
-                        uint32_t wa[WPL], wb[WPL];            // rows g and g + 8
-                        q4_words<WPL>(wrow + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wa);
-                        q4_words<WPL>(wrow + 8 * PITCH + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wb);
-                        float lo[NT][4], hi[NT][4];
+                        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+                    if (piece < pieces) {
+                        const uint32_t wrow = stage + (sub * 16 + g) * PITCH;
 #pragma unroll
-                        for (int j = 0; j < WPL; ++j) {
-                            uint32_t a[4], c[4];              // pairs (0,4) (1,5) (2,6) (3,7) of rows g and g + 8
-                            q4_pairs(wa[j], a);
-                            q4_pairs(wb[j], c);
+                        for (int gi = 0; gi < GC; ++gi) {
+                            uint32_t wa[WPL], wb[WPL];        // rows g and g + 8
+                            q4_words<WPL>(wrow + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wa);
+                            q4_words<WPL>(wrow + 8 * PITCH + ((gi * (GROUP / 2) + t * WPL * 4) ^ sw), wb);
+                            float lo[NT][4], hi[NT][4];
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const uint4 x = xr[gi * WPL + j][n];
-                                if (j == 0) {
-                                    mma_16816_first(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
-                                    mma_16816_first(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
-                                } else {
-                                    mma_16816(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
-                                    mma_16816(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
+                            for (int j = 0; j < WPL; ++j) {
+                                uint32_t a[4], c[4];          // pairs (0,4) (1,5) (2,6) (3,7) of rows g and g + 8
+                                q4_pairs(wa[j], a);
+                                q4_pairs(wb[j], c);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const uint4 x = xr[gi * WPL + j][n];
+                                    if (j == 0) {
+                                        mma_16816_first(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
+                                        mma_16816_first(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
+                                    } else {
+                                        mma_16816(lo[n], a[0], c[0], a[2], c[2], x.x, x.y);
+                                        mma_16816(hi[n], a[1], c[1], a[3], c[3], x.z, x.w);
+                                    }
                                 }
                             }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) { // i >> 1: row g or g + 8; i & 1: vector 2t or 2t + 1
+                                    float d = fmaf(hi[n][i], 0.0625f, lo[n][i]);
+                                    d = fmaf(nz[2 * sub + (i >> 1)][gi], xsum[gi][n][i & 1], d);
+                                    acc[n][i] = fmaf(sc[2 * sub + (i >> 1)][gi], d, acc[n][i]);
+                                }
                         }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {     // i >> 1: row g or g + 8; i & 1: vector 2t or 2t + 1
-                                float d = fmaf(hi[n][i], 0.0625f, lo[n][i]);
-                                d = fmaf(nz[i >> 1][gi], xsum[gi][n][i & 1], d);
-                                acc[n][i] = fmaf(sc[i >> 1][gi], d, acc[n][i]);
-                            }
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float* at = part + (n * 8 + (i & 1)) * RS + tile * TR + sub * 16 + (i >> 1) * 8;
+                            if (n * 8 + 2 * t + (i & 1) < p.n_vec) *at = pass == 0 ? acc[n][i] : *at + acc[n][i];
+                        }
                 }
-                stage += Cfg::TILE;
-                if (stage == ring + STAGES * Cfg::TILE) stage = ring;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t v = n * 8 + 2 * t + (i & 1);
-                        float* at = part + v * RS + tile * 16 + g + (i >> 1) * 8;
-                        if (v < p.n_vec) *at = pass == 0 ? acc[n][i] : *at + acc[n][i];
-                    }
+                stage = stage + Cfg::TILE == ring + STAGES * Cfg::TILE ? ring : stage + Cfg::TILE;
             }
         }
         // ---- join.  Two sets of partial sums: what the next block writes is not what this one reads.
@@ -442,23 +439,21 @@ gemv_q4_kernel(const GemvQ4Params p) {
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             join_cluster(b - per_join, per_join);
         }
-        float* const own = sums + ((b / per_join) & 1u) * Cfg::JOIN + in_join * R * p.n_vec;
-        for (uint32_t i = threadIdx.x; i < R * p.n_vec; i += blockDim.x) {
-            const float* at = parts + buf * warps * (Cfg::PART / 4) + i / R * RS + i % R;
+        float* const own = sums + ((b / per_join) & 1u) * Cfg::JOIN + in_join * block_sums;
+        for (uint32_t i = threadIdx.x; i < block_sums; i += blockDim.x) {
+            const float* at = parts + buf * warps * (Cfg::PART / 4) + i / Cfg::R * RS + i % Cfg::R;
             float s = 0.f;
             for (uint32_t w = 0; w < active; ++w) s += at[w * (Cfg::PART / 4)];
             if (ranks > 1) own[i] = s;
-            else store(block, i, s);
+            else store(b, i, s);
         }
-        if (ranks > 1 && (in_join + 1 == per_join || b + 1 == my_blocks))
+        if (ranks > 1 && (in_join + 1 == per_join || b + 1 == blocks))
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
     if (ranks > 1) {
-        if (my_blocks > 0) {
-            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-            const uint32_t b0 = (my_blocks - 1) / per_join * per_join;
-            join_cluster(b0, my_blocks - b0);
-        }
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const uint32_t b0 = (blocks - 1) / per_join * per_join;
+        join_cluster(b0, blocks - b0);
         cluster_sync_all();                                   // nobody leaves while its sums are being read
     }
 }
