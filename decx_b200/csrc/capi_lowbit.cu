@@ -146,7 +146,7 @@ int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, uns
     return 0;
 }
 
-constexpr uint32_t Q4_MAX_VEC = 16, Q4_MAX_RANKS = 8;
+constexpr uint32_t Q4_MAX_VEC = 16, Q4_MAX_RANKS = 16;
 
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
 int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
@@ -157,13 +157,17 @@ int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
     if (rc != 0) return rc;
     const uint32_t pieces = (p.cols + Cfg::KW - 1) / Cfg::KW;
     p.ranks = (pieces + Cfg::WARPS - 1) / Cfg::WARPS;
-    if (p.ranks > Q4_MAX_RANKS) p.ranks = Q4_MAX_RANKS;
-    uint32_t warps = (pieces + p.ranks - 1) / p.ranks;
-    if (warps > uint32_t(Cfg::WARPS)) warps = Cfg::WARPS;
-    p.passes = (pieces + p.ranks * warps - 1) / (p.ranks * warps);
+    if (p.ranks > Q4_MAX_RANKS) return DECXB200_ETOOLARGE;
+    const uint32_t warps = (pieces + p.ranks - 1) / p.ranks;
+    if (p.ranks > 8) {                       // beyond the portable cluster size
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return int(e);
+    }
     constexpr uint32_t GC = Cfg::KW / GROUP;
     p.vec_s = reinterpret_cast<uintptr_t>(p.scales) % (2 * GC) == 0 && p.lds % GC == 0;
     p.vec_z = reinterpret_cast<uintptr_t>(p.zeros) % GC == 0 && p.ldz % GC == 0;
+    constexpr uint32_t X = X8 ? 8 : 16;
+    p.vec_x = reinterpret_cast<uintptr_t>(p.x) % X == 0 && p.ldx % 8 == 0;
     // clusters the GPU holds at once: the grid, since they stay and take turns over the blocks of rows
     static std::atomic<int> held[Q4_MAX_RANKS][Cfg::WARPS];
     int clusters = held[p.ranks - 1][warps - 1].load(std::memory_order_relaxed);
@@ -173,7 +177,7 @@ int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
         cluster_config(cfg, attr, p.ranks, 32 * warps, Cfg::smem(warps), p.ranks, s);
         const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
         if (e != cudaSuccess) return int(e);
-        if (clusters < 1) clusters = 1;
+        if (clusters < 1) return DECXB200_ETOOLARGE;
         held[p.ranks - 1][warps - 1].store(clusters, std::memory_order_relaxed);
     }
     const uint64_t tiles = (uint64_t(p.rows) + Cfg::TR - 1) / Cfg::TR;
@@ -190,8 +194,19 @@ int run_gemv_q4(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) {
 template <int GROUP>
 int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) {
     const bool z = p.zeros != nullptr;
-    if (p.n_vec > 8) return z ? run_gemv_q4<GROUP, 2, true>(s, x8, f32, p) : run_gemv_q4<GROUP, 2, false>(s, x8, f32, p);
-    return z ? run_gemv_q4<GROUP, 1, true>(s, x8, f32, p) : run_gemv_q4<GROUP, 1, false>(s, x8, f32, p);
+    // Sixteen vectors at once take half as many columns per warp: with more than 16384 columns two rounds of eight do.
+    if (p.n_vec > 8 && p.cols <= 8 * Q4Cfg<2>::WARPS * Q4Cfg<2>::KW)
+        return z ? run_gemv_q4<GROUP, 2, true>(s, x8, f32, p) : run_gemv_q4<GROUP, 2, false>(s, x8, f32, p);
+    for (uint32_t v = 0; v < p.n_vec; v += 8) {
+        GemvQ4Params q = p;
+        q.n_vec = p.n_vec - v < 8 ? p.n_vec - v : 8;
+        q.x = static_cast<const uint8_t*>(p.x) + uint64_t(v) * p.ldx * (x8 ? 1 : 2);
+        q.y = static_cast<uint8_t*>(p.y) + uint64_t(v) * p.ldy * (f32 ? 4 : 2);
+        if (p.xs != nullptr) q.xs = p.xs + v;
+        const int rc = z ? run_gemv_q4<GROUP, 1, true>(s, x8, f32, q) : run_gemv_q4<GROUP, 1, false>(s, x8, f32, q);
+        if (rc != 0) return rc;
+    }
+    return 0;
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit GEMM
@@ -300,7 +315,8 @@ int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint
     const uint64_t groups = (uint64_t(cols) + group - 1) / group;
     if (ldw < (uint64_t(cols) + 1) / 2 || ld_scales < groups || (zeros != nullptr && ld_zeros < groups) || ldx < cols || ldy < rows)
         return DECXB200_EINVAL;
-    if (n_vec > Q4_MAX_VEC || cols > 0x7fffffffu || rows > 0x7fffffffu) return DECXB200_ETOOLARGE;
+    // columns that 16 CTAs hold; 32-bit offsets within a tile of 32 rows
+    if (n_vec > Q4_MAX_VEC || cols > 65536 || rows > 0x7fffff00u || ldw > (1u << 26) || ld_scales > (1u << 26) || ld_zeros > (1u << 26)) return DECXB200_ETOOLARGE;
     if (!aligned16(W) || (ldw % 16) != 0) return DECXB200_EALIGN;
     auto at = [](const void* a, uintptr_t e) { return (reinterpret_cast<uintptr_t>(a) & (e - 1)) == 0; };
     if (!at(scales, 2) || (x_dtype == DECXB200_FP16 && !at(x, 2)) || !at(x_scales, 4) || !at(y, y_dtype == DECXB200_FP32 ? 4 : 2))

@@ -283,9 +283,11 @@ DECXB200_API int decxb200_rmsnorm_q8(int dtype, void* stream, uint32_t rows, uin
  *   x:       n_vec x cols, fp16 or e4m3 (x_dtype DECXB200_FP16 / DECXB200_E4M3), ldx elements per vector.
  *   x_scales: n_vec fp32 factors (the scales of an 8-bit operand), or NULL: 1.
  *   y:       n_vec x rows, fp16 or fp32 (y_dtype), ldy elements per vector.
+ * Limits: 16 vectors, 65536 columns, pitches of W, scales and zeros of 2^26; beyond them DECXB200_ETOOLARGE.
  * Products q x are exact; sums of q x and of x over a group, their combination with z and the scales are fp32, and an
- * fp16 y is rounded once.  A vector that holds a NaN or an infinity gives NaN.  The weights are read once whatever
- * n_vec is.  Partial sums are added in a fixed order: results do not depend on timing.  Asynchronous on `stream`.
+ * fp16 y is rounded once.  A vector that holds a NaN or an infinity gives NaN.  The weights are read once
+ * whatever n_vec is (twice for more than 8 vectors and more than 16384 columns).  Partial sums are added in a fixed
+ * order: results do not depend on timing.  Asynchronous on `stream`.
  */
 DECXB200_API int decxb200_gemv_q4(int x_dtype, int y_dtype, void* stream, uint32_t rows, uint32_t cols, uint32_t n_vec,
                                   uint32_t group, const void* W, uint64_t ldw, const void* scales, uint64_t ld_scales,

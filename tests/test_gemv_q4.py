@@ -9,7 +9,8 @@ E4M3 = torch.float8_e4m3fn
 
 # one row, one column, part of a row block, several; part of a group, of a slice, several slices, more than a cluster holds
 SHAPES = [(1, 1), (1, 32), (5, 31), (64, 33), (65, 64), (63, 513), (130, 1000), (200, 2049), (64, 4099), (300, 8192),
-          (70, 16384), (9, 20001), (4800, 544), (20000, 1056)]
+          (70, 16384), (9, 20001), (33, 40000), (17, 65536), (4800, 544),
+          (20000, 1056)]
 
 
 @pytest.fixture(scope="module")
@@ -171,7 +172,7 @@ def test_refusals_of_the_c_abi():
     assert call(W=None) == -1 and call(s=None) == -1 and call(x=None) == -1 and call(y=None) == -1
     assert call(group=16) == -1 and call(group=0) == -1 and call(group=256) == -1
     assert call(ldw=16) == -1 and call(lds=1) == -1 and call(z=p, ldz=1) == -1 and call(ldx=63) == -1 and call(ldy=3) == -1
-    assert call(n=17) == -5
+    assert call(n=17) == -5 and call(cols=65537, ldw=32784, lds=2049, ldx=65537) == -5 and call(ldw=1 << 27) == -5
     assert call(W=p + 8) == -2 and call(ldw=40) == -2 and call(s=p + 1) == -2 and call(x=p + 1) == -2
     assert call(y=p + 2) == -2 and call(xs=p + 2) == -2
 
