@@ -662,7 +662,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_const
                     bool arrived = true, waited = false;
                     while (int(ld_acquire_sys(p.panel_flags + panel) - p.panel_epoch) < 0) {
                         waited = true;
-                        if (global_timer_ns() - t0 > limit) { arrived = false; break; }
+                        // a little less patient than the MMA thread, which waits for this loader: the code that is
+                        // reported names the panel
+                        if (global_timer_ns() - t0 > limit - limit / 8) { arrived = false; break; }
                     }
                     if (waited && p.stats != nullptr) {
                         atomicAdd(p.stats + 18, (unsigned long long)(global_timer_ns() - t0));
