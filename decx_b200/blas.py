@@ -9,8 +9,8 @@ import ctypes
 
 import torch
 
-from . import capi
-from .gemm import _ld, _on, _stream
+from . import _front, capi
+from .gemm import _ld
 
 _OUT = {(capi.FP32, 0): torch.float32, (capi.FP16, capi.ACCU_L1): torch.float32,
         (capi.FP16, capi.ACCU_L2): torch.float16, (capi.FP16, capi.ACCU_L3): torch.float16}
@@ -77,9 +77,6 @@ def cast(src, dtype, out=None):
     return out
 
 
-_Q8_IN = {torch.float16: capi.FP16, torch.float32: capi.FP32}
-
-
 def new_q8(rows, cols, device):
     """An empty 8-bit operand: a rows x cols float8_e4m3fn view whose rows start a multiple of 128 bytes apart
     (the layout ``gemm.gemm_q8`` takes), and its rows' float32 scales."""
@@ -88,31 +85,19 @@ def new_q8(rows, cols, device):
 
 
 def _q8_out(src, out, scales):
-    if out is None or scales is None:
-        q, s = new_q8(src.shape[0], src.shape[1], src.device)
-        out, scales = (q if out is None else out), (s if scales is None else scales)
-    if out.dtype != torch.float8_e4m3fn or out.shape != src.shape or out.device != src.device:
-        raise ValueError("out must be a float8_e4m3fn matrix of the input's shape on its device")
-    if scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != src.shape[0] or not scales.is_contiguous() \
-            or scales.device != src.device:
-        raise ValueError("scales must be a contiguous float32 vector with one entry per row")
-    return out, scales
+    rows, cols = src.shape
+    q, s = new_q8(rows, cols, src.device)
+    return (q if out is None else out), (s if scales is None else scales)
 
 
 def cast_q8(src, out=None, scales=None):
     """``src`` (rows x cols, float16 or float32, pitched) as an 8-bit operand: returns ``(q, scales)`` with
     ``scales[r] = max|src[r]| / 448`` and ``q = e4m3(src / scales[:, None])``.  Launches on torch's current stream."""
-    if not src.is_cuda:
-        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
-    dt = _Q8_IN.get(src.dtype)
-    if dt is None:
-        raise TypeError("cast_q8 takes float16 or float32")
-    lds = _ld(src)
-    out, scales = _q8_out(src, out, scales)
-    dev = src.device
-    rows, cols = src.shape
-    _on(dev, capi.lib.decxb200_cast_q8, dt, _stream(dev), rows, cols, src.data_ptr(), lds, out.data_ptr(), _ld(out),
-        scales.data_ptr())
+    if out is None or scales is None:
+        out, scales = _q8_out(src, out, scales)
+    code = _front.cast_q8(src, out, scales)
+    if code:
+        capi.check(code)
     return out, scales
 
 
@@ -122,30 +107,13 @@ def rmsnorm_q8(x, weight, residual=None, eps=1e-6, out=None, scales=None, sum_ou
     ``h = x + residual``, ``sum = h`` rounded to x's type (None without a residual), ``y = h / sqrt(mean(h^2) + eps) *
     weight``, ``scales[r] = max|y[r]| / 448``, ``q = e4m3(y / scales[:, None])``.  float16 or float32, pitched rows;
     ``sum_out`` may be ``x`` or ``residual`` themselves.  Launches on torch's current stream."""
-    if not x.is_cuda:
-        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
-    dt = _Q8_IN.get(x.dtype)
-    if dt is None or weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
-        raise TypeError("x, weight and residual must share one dtype out of float16, float32")
-    ldx, dev = _ld(x), x.device
-    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or not weight.is_contiguous() or weight.device != dev:
-        raise ValueError("weight must be a contiguous vector with one entry per column of x")
-    if residual is None:
-        if sum_out is not None:
-            raise ValueError("sum_out without a residual")
-    else:
-        if residual.shape != x.shape or residual.device != dev:
-            raise ValueError("residual must have the shape of x")
-        if sum_out is None:
-            sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif sum_out.shape != x.shape or sum_out.dtype != x.dtype or sum_out.device != dev:
-            raise ValueError("sum_out must have the shape and type of x")
-    out, scales = _q8_out(x, out, scales)
-    rows, cols = x.shape
-    _on(dev, capi.lib.decxb200_rmsnorm_q8, dt, _stream(dev), rows, cols, x.data_ptr(), ldx,
-        residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
-        sum_out.data_ptr() if sum_out is not None else None, _ld(sum_out) if sum_out is not None else 0,
-        weight.data_ptr(), eps, out.data_ptr(), _ld(out), scales.data_ptr())
+    if out is None or scales is None:
+        out, scales = _q8_out(x, out, scales)
+    if sum_out is None and residual is not None:
+        sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    code = _front.rmsnorm_q8(x, weight, residual, eps, out, scales, sum_out)
+    if code:
+        capi.check(code)
     return out, scales, sum_out
 
 
@@ -167,35 +135,12 @@ def gemv_q4(W, scales, x, group, zeros=None, x_scales=None, out_dtype=torch.floa
     ``(q - zeros[r, k // group]) * scales[r, k // group]``, with 8 for the zero when ``zeros`` is None.  ``scales``:
     float16; ``zeros``: uint8; ``group``: 32, 64 or 128.  ``x``: float16, or float8_e4m3fn whose rows stand for
     ``x * x_scales[:, None]``.  Sums are float32.  Launches on torch's current stream."""
-    if not W.is_cuda:
-        raise RuntimeError("decx_b200.blas works on CUDA tensors only (no CPU fallback)")
-    if W.dtype != torch.uint8 or scales.dtype != torch.float16 or (zeros is not None and zeros.dtype != torch.uint8):
-        raise TypeError("gemv_q4 takes uint8 W, float16 scales and uint8 zeros")
-    xt = {torch.float16: capi.FP16, torch.float8_e4m3fn: capi.E4M3}.get(x.dtype)
-    if xt is None:
-        raise TypeError("x must be float16 or float8_e4m3fn")
-    single = x.dim() == 1
-    xm = x[None] if single else x
-    ldx, ldw, lds = _ld(xm), _ld(W), _ld(scales)
-    n, cols = xm.shape
-    rows = W.shape[0]
-    groups = -(-cols // group) if group > 0 else 0
-    if W.shape[1] != (cols + 1) // 2 or scales.shape != (rows, groups) or (zeros is not None and zeros.shape != (rows, groups)):
-        raise ValueError("W is rows x ceil(cols / 2), scales and zeros rows x ceil(cols / group), x vectors of cols entries")
-    if x_scales is not None and (x_scales.dtype != torch.float32 or x_scales.numel() != n or not x_scales.is_contiguous()):
-        raise ValueError("x_scales must be contiguous float32 with one entry per vector")
     if out is None:
-        out = torch.empty(rows if single else (n, rows), dtype=out_dtype, device=W.device)
-    yt = {torch.float16: capi.FP16, torch.float32: capi.FP32}.get(out.dtype)
-    ym = out[None] if single else out
-    if yt is None or ym.shape != (n, rows):
-        raise ValueError("the result is float16 or float32, one entry per row of W for each vector")
-    dev = W.device
-    if any(a is not None and a.device != dev for a in (scales, zeros, x, x_scales, out)):
-        raise ValueError("all operands must be on one device")
-    _on(dev, capi.lib.decxb200_gemv_q4, xt, yt, _stream(dev), rows, cols, n, group, W.data_ptr(), ldw, scales.data_ptr(), lds,
-        zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else 0, xm.data_ptr(), ldx,
-        x_scales.data_ptr() if x_scales is not None else None, ym.data_ptr(), _ld(ym))
+        rows = W.shape[0]
+        out = torch.empty(rows if x.dim() == 1 else (x.shape[0], rows), dtype=out_dtype, device=W.device)
+    code = _front.gemv_q4(W, scales, x, group, zeros, x_scales, out)
+    if code:
+        capi.check(code)
     return out
 
 

@@ -60,6 +60,26 @@ def build_host(force=False):
     return out
 
 
+FRONT = os.path.join(HERE, "front")
+
+
+def build_front(force=False):
+    """The Python entry of the low-precision operators (front/front.cpp): decx_b200/_front.so, against this torch."""
+    import sysconfig
+    import torch
+    out, src = os.path.join(HERE, "_front.so"), os.path.join(FRONT, "front.cpp")
+    tdir = os.path.dirname(torch.__file__)
+    if force or _stale(out, [src, os.path.join(ROOT, "include", "decx_b200.h")]):
+        cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I", sysconfig.get_paths()["include"], "-I", os.path.join(tdir, "include"),
+               "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(CUDA_HOME, "include"),
+               src, "-o", out, "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+               "-L", CSRC, "-ldecx_b200", "-Wl,-rpath,$ORIGIN/csrc"]
+        subprocess.run(cmd, check=True, cwd=FRONT)
+    return out
+
+
 def build_cpp_tests(force=False):
     """The C++ programs under tests/cpp (written against include/DECX.h like a DECX user program)."""
     tdir = os.path.join(ROOT, "tests", "cpp")
@@ -83,7 +103,7 @@ def build_cpp_tests(force=False):
 
 
 def build_all(force=False, verbose=False):
-    return [build_kernels(force, verbose), build_host(force)] + build_cpp_tests(force)
+    return [build_kernels(force, verbose), build_host(force), build_front(force)] + build_cpp_tests(force)
 
 
 if __name__ == "__main__":

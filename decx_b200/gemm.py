@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from . import capi
+from . import _front, capi
 
 _DTYPES = {torch.float32: capi.FP32, torch.float16: capi.FP16, torch.complex64: capi.CPLXF,
            torch.float64: capi.FP64, torch.complex128: capi.CPLXD}
@@ -20,21 +20,6 @@ def _ld(t):
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError("matrices must be 2-D with unit column stride (row-major, pitched)")
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
-
-
-def _on(device, fn, *args):
-    """Calls a launching entry point with `device` current.  Switching the device (and building a Stream object, see
-    `_stream`) costs more host time than a small launch, so neither is done when it is not needed."""
-    if device.index == torch.cuda.current_device():
-        capi.check(fn(*args))
-    else:
-        with torch.cuda.device(device):
-            capi.check(fn(*args))
-
-
-def _stream(device):
-    """Handle of torch's current stream of `device`."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _scalar(dtype, v):
@@ -97,31 +82,11 @@ def gemm_q8(A, scale_a, B, scale_b, C=None, alpha=None, beta=None, out=None, out
     ``scale_a`` / ``scale_b`` their rows' float32 scales: what ``blas.cast_q8`` and ``blas.rmsnorm_q8`` return.  ``C``
     and the result are float16 or float32 (``out_dtype``); ``C`` may be ``out``.  Sums are float32.  Launches on torch's
     current stream of A's device; returns ``out`` (asynchronous)."""
-    if not A.is_cuda:
-        raise RuntimeError("decx_b200.gemm works on CUDA tensors only (no CPU fallback)")
-    if A.dtype != torch.float8_e4m3fn or B.dtype != torch.float8_e4m3fn:
-        raise TypeError("A and B must be float8_e4m3fn")
-    M, K = A.shape
-    N, K2 = B.shape
-    if K2 != K:
-        raise ValueError(f"A is {M}x{K} but B is {N}x{K2}")
-    dev = A.device
-    for v, n in ((scale_a, M), (scale_b, N)):
-        if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != n or not v.is_contiguous():
-            raise ValueError("scale_a and scale_b must be contiguous float32 vectors with one entry per row of A / B")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype if C is None else C.dtype, device=dev)
-    dt = {torch.float16: capi.FP16, torch.float32: capi.FP32}.get(out.dtype)
-    if dt is None or (C is not None and C.dtype != out.dtype):
-        raise TypeError("C and the result must share one dtype out of float16, float32")
-    if out.shape != (M, N) or (C is not None and C.shape != (M, N)):
-        raise ValueError("C and out must be M x N")
-    if any(t is not None and t.device != dev for t in (B, scale_a, scale_b, C, out, status)):
-        raise ValueError("all operands must be on one device")
-    _on(dev, capi.lib.decxb200_gemm_q8, dt, _stream(dev), M, N, K, A.data_ptr(), _ld(A), scale_a.data_ptr(), B.data_ptr(), _ld(B),
-        scale_b.data_ptr(), C.data_ptr() if C is not None else None, _ld(C) if C is not None else 0, out.data_ptr(), _ld(out),
-        ctypes.c_float(alpha) if alpha is not None else None, ctypes.c_float(beta) if beta is not None and C is not None else None,
-        status.data_ptr() if status is not None else None, tile)
+        out = torch.empty((A.shape[0], B.shape[0]), dtype=out_dtype if C is None else C.dtype, device=A.device)
+    code = _front.gemm_q8(A, scale_a, B, scale_b, C, alpha, beta, out, status, tile)
+    if code:
+        capi.check(code)
     return out
 
 
