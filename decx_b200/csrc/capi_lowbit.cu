@@ -16,9 +16,45 @@ using dxb_host::round_up;
 
 namespace {
 
-inline int last_error() {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : int(e);
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    return n;
+}
+
+// Launch configuration with a cluster of CTAs.  All kernels here wait for the grids before them themselves
+// (griddep_wait), so they are launched programmatically dependent on them: their CTAs start while the last ones of the
+// previous kernel drain.  DECXB200_PDL=0 turns that off.
+void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], unsigned blocks, unsigned threads, unsigned smem,
+                    unsigned cluster, cudaStream_t s) {
+    static const int pdl_env = [] { const char* e = getenv("DECXB200_PDL"); return e ? atoi(e) : 1; }();
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    if (pdl_env != 0) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+}
+
+template <typename K, typename... Args>
+int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    cluster_config(cfg, attr, blocks, threads, smem, cluster, s);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) return int(e);
+    dxb_host::count_launch();
+    return 0;
 }
 
 // Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device.
@@ -32,12 +68,6 @@ int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
     if (e != cudaSuccess) return int(e);
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
     return 0;
-}
-
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-    return n;
 }
 
 template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
@@ -66,9 +96,7 @@ int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
     const uint32_t per_sm = by_smem < most ? by_smem : most;
     const uint64_t want = WARP ? (uint64_t(p.rows) + threads / 32 - 1) / (threads / 32) : p.rows;
     const uint64_t have = uint64_t(sm_count()) * (per_sm ? per_sm : 1);
-    kern<<<unsigned(want < have ? want : have), threads, row * p.depth, s>>>(p);
-    dxb_host::count_launch();
-    return last_error();
+    return launch_cluster(kern, unsigned(want < have ? want : have), threads, row * p.depth, 1, s, p);
 }
 
 // kernels that keep one row per CTA or warp: few rows (no ring to fill), or operands that only single elements fit
@@ -76,20 +104,17 @@ template <typename T, bool NORM, bool VEC>
 int launch_row_q8(cudaStream_t s, const RowQ8Params& p) {
     if (p.cols <= 1024) {
         const unsigned blocks = unsigned((uint64_t(p.rows) + 7) / 8);
-        if (p.cols <= 256) row_q8_kernel<T, NORM, true, VEC, 1><<<blocks, 256, 0, s>>>(p);
-        else if (p.cols <= 512) row_q8_kernel<T, NORM, true, VEC, 2><<<blocks, 256, 0, s>>>(p);
-        else row_q8_kernel<T, NORM, true, VEC, 4><<<blocks, 256, 0, s>>>(p);
-    } else {
-        const unsigned blocks = p.rows < 0x7fffffffu ? p.rows : 0x7fffffffu;
-        const uint32_t chunks = (p.cols + 7) / 8;
-        auto threads = [&](uint32_t nch) { return (chunks + 32 * nch - 1) / (32 * nch) * 32; };
-        if (p.cols > 8 * 4 * 1024) row_q8_long_kernel<T, NORM><<<blocks, 1024, 0, s>>>(p);
-        else if (chunks <= 1024 && p.rows <= 296) row_q8_kernel<T, NORM, false, VEC, 1><<<blocks, threads(1), 0, s>>>(p);
-        else if (chunks <= 2048) row_q8_kernel<T, NORM, false, VEC, 2><<<blocks, threads(2), 0, s>>>(p);
-        else row_q8_kernel<T, NORM, false, VEC, 4><<<blocks, threads(4), 0, s>>>(p);
+        if (p.cols <= 256) return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 1>, blocks, 256, 0, 1, s, p);
+        if (p.cols <= 512) return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 2>, blocks, 256, 0, 1, s, p);
+        return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 4>, blocks, 256, 0, 1, s, p);
     }
-    dxb_host::count_launch();
-    return last_error();
+    const unsigned blocks = p.rows < 0x7fffffffu ? p.rows : 0x7fffffffu;
+    const uint32_t chunks = (p.cols + 7) / 8;
+    auto threads = [&](uint32_t nch) { return (chunks + 32 * nch - 1) / (32 * nch) * 32; };
+    if (p.cols > 8 * 4 * 1024) return launch_cluster(row_q8_long_kernel<T, NORM>, blocks, 1024, 0, 1, s, p);
+    if (chunks <= 1024 && p.rows <= 296) return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 1>, blocks, threads(1), 0, 1, s, p);
+    if (chunks <= 2048) return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 2>, blocks, threads(2), 0, 1, s, p);
+    return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 4>, blocks, threads(4), 0, 1, s, p);
 }
 
 template <typename T, bool NORM, bool RES, bool SHIFT>
@@ -120,32 +145,6 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     return rows16 ? launch_row_q8_shape<T, NORM, false, false>(s, p) : launch_row_q8_shape<T, NORM, false, true>(s, p);
 }
 
-void cluster_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[1], unsigned blocks, unsigned threads, unsigned smem,
-                    unsigned cluster, cudaStream_t s) {
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-}
-
-template <typename K, typename... Args>
-int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t s, const Args&... args) {
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr[1];
-    cluster_config(cfg, attr, blocks, threads, smem, cluster, s);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-    if (e != cudaSuccess) return int(e);
-    dxb_host::count_launch();
-    return 0;
-}
-
 constexpr uint32_t Q4_MAX_VEC = 16, Q4_MAX_RANKS = 16;
 
 template <int GROUP, int NT, bool ZEROS, bool X8, typename OUT>
@@ -172,10 +171,16 @@ int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
     static std::atomic<int> held[Q4_MAX_RANKS][Cfg::WARPS];
     int clusters = held[p.ranks - 1][warps - 1].load(std::memory_order_relaxed);
     if (clusters == 0) {
-        cudaLaunchConfig_t cfg;
-        cudaLaunchAttribute attr[1];
-        cluster_config(cfg, attr, p.ranks, 32 * warps, Cfg::smem(warps), p.ranks, s);
-        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+        cudaError_t e;
+        if (p.ranks == 1) {
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&clusters, kern, int(32 * warps), Cfg::smem(warps));
+            clusters *= sm_count();
+        } else {
+            cudaLaunchConfig_t cfg;
+            cudaLaunchAttribute attr[2];
+            cluster_config(cfg, attr, p.ranks, 32 * warps, Cfg::smem(warps), p.ranks, s);
+            e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+        }
         if (e != cudaSuccess) return int(e);
         if (clusters < 1) return DECXB200_ETOOLARGE;
         held[p.ranks - 1][warps - 1].store(clusters, std::memory_order_relaxed);

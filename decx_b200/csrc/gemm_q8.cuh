@@ -176,6 +176,8 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_alloc<1>(slot, Cfg::TMEM_COLS);
         tmem_relinquish<1>();
     }
+    griddep_launch();
+    griddep_wait();                                                   // nothing of the operands is touched before
     if (warp >= 2 && threadIdx.x - 64 < BN) {
         const uint32_t m = tm * BN + threadIdx.x - 64;
         sa[threadIdx.x - 64] = m < p.M ? p.sa[m] : 0.f;
@@ -399,6 +401,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_alloc<2>(slot, 512);
         tmem_relinquish<2>();
     }
+    griddep_launch();
+    griddep_wait();                                                   // nothing of the operands is touched before
     tc_fence_before_sync();
     cluster_sync_all();
     tc_fence_after_sync();

@@ -227,6 +227,8 @@ gemv_q4_kernel(const GemvQ4Params p) {
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     static_assert((STAGES & (STAGES - 1)) == 0, "the ring wraps by a mask");
+    griddep_launch();
+    griddep_wait();
     for (int d = 0; d < STAGES - 1; ++d) request(d, d * Cfg::TILE);
 
     // ---- scales and zero points of rows g, g + 8, ... of a tile, asked for one tile ahead

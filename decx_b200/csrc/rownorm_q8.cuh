@@ -122,6 +122,8 @@ row_q8_kernel(const RowQ8Params p) {
     const uint32_t tpr = WARP ? 32u : blockDim.x;
     const uint32_t tid = WARP ? (threadIdx.x & 31u) : threadIdx.x;
     const uint32_t row_step = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+    griddep_launch();
+    griddep_wait();
     const T* w = static_cast<const T*>(p.w);
     for (uint32_t row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x; row < p.rows; row += row_step) {
         const T* x = static_cast<const T*>(p.x) + uint64_t(row) * p.ldx;
@@ -324,6 +326,8 @@ row_q8_ring_kernel(const RowQ8Params p) {
     const uint32_t unit_bytes = warps * WARP_BYTES, slot_bytes = unit_bytes * NC * MATS;
     const uint32_t mine = smem_u32(q8_ring) + wid * WARP_BYTES + lane * 16;
     const int32_t row_bytes = int32_t(p.cols * sizeof(T));
+    griddep_launch();
+    griddep_wait();
 
     // what stays the same for every row: the thread's first bytes, and its pieces of the weight
     uint32_t w[NORM ? NC : 1][4];
@@ -516,6 +520,8 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(const RowQ8Params p) 
     __shared__ float red_ss[32];
     __shared__ uint32_t red_top[32];
     const T* w = static_cast<const T*>(p.w);
+    griddep_launch();
+    griddep_wait();
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const T* x = static_cast<const T*>(p.x) + uint64_t(row) * p.ldx;
         const T* r = p.r != nullptr ? static_cast<const T*>(p.r) + uint64_t(row) * p.ldr : nullptr;
