@@ -215,42 +215,53 @@ int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) 
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit GEMM
+template <int BN, bool SPLIT, typename T>
+int launch_q8_thin(cudaStream_t s, const GemmQ8Params& p, const CUtensorMap& ma, const CUtensorMap& mb) {
+    using Cfg = ThinCfg<BN, SPLIT>;
+    auto kern = gemm_q8_thin_kernel<BN, SPLIT, T>;
+    static std::atomic<uint64_t> done{0};
+    const int rc = allow_smem(kern, Cfg::SMEM_BYTES, done);
+    if (rc != 0) return rc;
+    const uint64_t blocks = uint64_t(p.tiles_m) * p.tiles_n * p.ranks;
+    if (blocks > 0x7fffffffull) return DECXB200_ETOOLARGE;
+    return launch_cluster(kern, unsigned(blocks), 192, Cfg::SMEM_BYTES, p.ranks, s, ma, mb, p);
+}
+
 template <int BN, typename T>
-int launch_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
-    using Cfg = ThinCfg<BN>;
+int run_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
     CUtensorMap ma, mb;
     int rc;
     if ((rc = dxb_host::tensor_map_2d(&ma, 1, A, p.M, p.K, lda, Q8_KB, BN)) != 0) return rc;
     if ((rc = dxb_host::tensor_map_2d(&mb, 1, B, p.N, p.K, ldb, Q8_KB, 128)) != 0) return rc;
-    auto kern = gemm_q8_thin_kernel<BN, T>;
-    static std::atomic<uint64_t> done{0};
-    if ((rc = allow_smem(kern, Cfg::SMEM_BYTES, done)) != 0) return rc;
     p.tiles_m = (p.M + BN - 1) / BN;
     p.tiles_n = (p.N + 127) / 128;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     const uint32_t n_kb = (p.K + Q8_KB - 1) / Q8_KB;
-    p.vec_d = (reinterpret_cast<uintptr_t>(p.D) % (4 * sizeof(T))) == 0 && p.ldd % 4 == 0;
+    // cut K until the GPU is full (two CTAs per SM; BN 128: one), at least two stages each
+    const uint64_t room = BN == 128 ? 148 : 296;
     p.ranks = 1;
-    while (p.ranks < 8 && tiles * p.ranks * 2 <= 296 && n_kb >= p.ranks * 2 * 4) p.ranks *= 2;
-    if (tiles * p.ranks > 0x7fffffffull) return DECXB200_ETOOLARGE;
-    return launch_cluster(kern, unsigned(tiles * p.ranks), 192, Cfg::SMEM_BYTES, p.ranks, s, ma, mb, p);
+    while (p.ranks < 8 && tiles * p.ranks * 2 <= room && n_kb >= p.ranks * 2 * 2) p.ranks *= 2;
+    return p.ranks > 1 ? launch_q8_thin<BN, true, T>(s, p, ma, mb) : launch_q8_thin<BN, false, T>(s, p, ma, mb);
 }
 
 template <typename T>
 int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, const void* B, uint64_t ldb) {
-    CUtensorMap ma, mb, md;
+    using Cfg = PairCfg;
+    CUtensorMap ma, mb, md, mc;
     int rc;
     if ((rc = dxb_host::tensor_map_2d(&ma, 1, A, p.M, p.K, lda, Q8_KB, 128)) != 0) return rc;
     if ((rc = dxb_host::tensor_map_2d(&mb, 1, B, p.N, p.K, ldb, Q8_KB, 128)) != 0) return rc;
-    md = ma;
+    md = mc = ma;
     const uint64_t e = sizeof(T);
     if (aligned16(p.D) && (p.ldd * e) % 16 == 0 &&
-        dxb_host::tensor_map_2d(&md, int(e), p.D, p.M, p.N, p.ldd, uint32_t(128 / e), 32) == 0)
+        dxb_host::tensor_map_2d(&md, int(e), p.D, p.M, p.N, p.ldd, uint32_t(64 / e), 32) == 0)
         p.d_tma = 1;
-    p.vec_c = p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0;
+    if (p.d_tma && p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0 &&
+        dxb_host::tensor_map_2d(&mc, int(e), p.C, p.M, p.N, p.ldc, uint32_t(64 / e), 32) == 0)
+        p.c_tma = 1;
     auto kern = gemm_q8_pair_kernel<T>;
     static std::atomic<uint64_t> done{0};
-    if ((rc = allow_smem(kern, PairCfg::SMEM_BYTES, done)) != 0) return rc;
+    if ((rc = allow_smem(kern, Cfg::SMEM_BYTES, done)) != 0) return rc;
     p.tiles_m = uint32_t((uint64_t(p.M) + 255) / 256);
     p.tiles_n = uint32_t((uint64_t(p.N) + 255) / 256);
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
@@ -259,7 +270,7 @@ int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
     uint64_t pairs = uint64_t(sm_count()) / 2;
     if (pairs > tiles) pairs = tiles;
     if (pairs == 0) pairs = 1;
-    return launch_cluster(kern, unsigned(2 * pairs), PairCfg::THREADS, PairCfg::SMEM_BYTES, 2, s, ma, mb, md, p);
+    return launch_cluster(kern, unsigned(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, 2, s, ma, mb, md, mc, p);
 }
 
 template <typename T>
@@ -269,10 +280,10 @@ int run_gemm_q8(cudaStream_t s, const GemmQ8Params& p, const void* A, uint64_t l
         tile = p.M > 128 && tiles >= 48 ? DECXB200_TILE_Q8_PAIR : DECXB200_TILE_Q8_THIN;
     }
     if (tile == DECXB200_TILE_Q8_PAIR) return launch_q8_pair<T>(s, p, A, lda, B, ldb);
-    if (p.M <= 16) return launch_q8_thin<16, T>(s, p, A, lda, B, ldb);
-    if (p.M <= 32) return launch_q8_thin<32, T>(s, p, A, lda, B, ldb);
-    if (p.M <= 64) return launch_q8_thin<64, T>(s, p, A, lda, B, ldb);
-    return launch_q8_thin<128, T>(s, p, A, lda, B, ldb);
+    if (p.M <= 16) return run_q8_thin<16, T>(s, p, A, lda, B, ldb);
+    if (p.M <= 32) return run_q8_thin<32, T>(s, p, A, lda, B, ldb);
+    if (p.M <= 64) return run_q8_thin<64, T>(s, p, A, lda, B, ldb);
+    return run_q8_thin<128, T>(s, p, A, lda, B, ldb);
 }
 
 }  // namespace
@@ -286,7 +297,7 @@ int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_t N, uint32_t
     if (d_dtype != DECXB200_FP16 && d_dtype != DECXB200_FP32) return DECXB200_EINVAL;
     if (A == nullptr || B == nullptr || D == nullptr || a_scales == nullptr || b_scales == nullptr) return DECXB200_EINVAL;
     if (M == 0 || N == 0 || K == 0 || lda < K || ldb < K || ldd < N || (C != nullptr && ldc < N)) return DECXB200_EINVAL;
-    if (tile != DECXB200_TILE_AUTO && tile != DECXB200_TILE_Q8_THIN && tile != DECXB200_TILE_Q8_PAIR) return DECXB200_EINVAL;
+    if (tile < DECXB200_TILE_AUTO || tile > DECXB200_TILE_Q8_PAIR) return DECXB200_EINVAL;
     if (M > 0x7fffff00u || N > 0x7fffff00u || K > 0x7fffff00u) return DECXB200_ETOOLARGE;   // TMA coordinates are signed
     if (!aligned16(A) || !aligned16(B) || (lda % 16) != 0 || (ldb % 16) != 0) return DECXB200_EALIGN;
     const uintptr_t e = d_dtype == DECXB200_FP16 ? 2 : 4;

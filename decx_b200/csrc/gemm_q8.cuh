@@ -5,17 +5,20 @@
 // TMA with the 128-byte swizzle.  The scales are applied to the finished fp32 sums in the epilogue.
 //
 // Two kernels:
-//   gemm_q8_pair   large products: persistent CTA pairs (cta_group::2), 256 x 256 tiles, two TMEM accumulators so that
-//                  one tile's epilogue runs under the next tile's MMAs.  The pair form halves what each SM's shared
-//                  memory has to deliver per MMA: each CTA holds its own 128 rows of A and of B only.
+//   gemm_q8_pair   large products: persistent CTA pairs (cta_group::2) on tiles of 256 x 256, two TMEM accumulators so
+//                  that one tile's epilogue runs under the next tile's MMAs.  The pair form halves what each SM's shared
+//                  memory has to deliver per MMA: each CTA holds its own 128 rows of A and of B only.  What bounds it is
+//                  that memory: 64 bytes per clock read by the MMAs and 64 written by TMA at the full rate.  One 128 of K
+//                  takes 660 clocks in a long run, 512 at that rate.  (256 x 512 tiles, two accumulators sharing A, were
+//                  measured: 2048 x 16384 x 4096 118 us against 102, 2048 x 4096 x 16384 99 against 102.)
 //   gemm_q8_thin   few rows of A (tokens) or few tiles: the operands swap places.  128 rows of B (weights) fill the
 //                  128 lanes of the MMA whatever M is, and the rows of A are its N side, 16 to 128 at a time.  Such
-//                  products are bound by reading B, so K is cut over a cluster of up to 8 CTAs until the GPU is full;
-//                  the cluster adds its partial tiles through distributed shared memory in rank order: one launch,
-//                  no workspace, no atomics.
+//                  products are bound by reading B, so K is cut over a cluster of up to 8 CTAs until the GPU is full.
+//                  Each CTA then sends its partial sums into the shared memory of the CTA that finishes these tokens
+//                  (st.async, counted by an mbarrier there), which adds them in rank order: one launch, no workspace,
+//                  no atomics, and no barrier that everybody has to reach at the end.
 // Every wait is bounded: on time-out the role writes a code to *status and the kernel unwinds.
 #pragma once
-#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include "sm100_ptx.cuh"
 
@@ -29,9 +32,8 @@ struct GemmQ8Params {
     void* D;
     uint64_t ldc, ldd;
     float alpha, beta;
-    int vec_d;                 // thin kernel: four neighbouring elements of D may be written at once
     int d_tma;                 // pair kernel: D through a staging tile and TMA stores (tmD); else per-thread stores
-    int vec_c;                 // pair kernel: rows of C are 16-byte aligned
+    int c_tma;                 // pair kernel: boxes of C through TMA loads (tmC), into the same buffers
     uint32_t tiles_m, tiles_n;
     uint32_t group_m;          // pair kernel: height of the rasterisation groups, in tiles
     uint32_t ranks;            // thin kernel: CTAs that share a tile's K = cluster size
@@ -77,83 +79,126 @@ __device__ __forceinline__ void q8_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void q8_put(__half* p, float v) { *p = __float2half_rn(v); }
 
 // =============================================================================================== thin kernel
-template <int BN>
+template <int BN, bool SPLIT>
 struct ThinCfg {
     static constexpr uint32_t STAGE = Q8_TILE + BN * Q8_KB;
-    static constexpr int STAGES = (108 * 1024) / STAGE;               // two CTAs per SM
+    // two CTAs per SM; 128 tokens with the inbox: one
+    static constexpr int STAGES = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 3 : (SPLIT ? 5 : 3);
     static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + 1024 /*alignment slack*/ + 256 /*barriers*/ + BN * 4 /*scales of A*/;
+    static constexpr uint32_t INBOX = SPLIT ? BN * 512 : 0;           // partial sums of this CTA's tokens, from all ranks
+    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + 1024 /*alignment slack*/ + 256 /*barriers*/ + BN * 4 /*scales of A*/ + INBOX;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 128, BN);
-    static_assert(STAGES * STAGE >= 128 * BN * 4, "the partial tile is exchanged in the ring");
-    static_assert(16 * STAGES + 16 <= 256, "barrier area");
+    static_assert(16 * STAGES + 24 <= 256, "barrier area");
 };
 
-// four neighbouring columns of one row of D
-template <typename T>
-__device__ __forceinline__ void q8_put4(const GemmQ8Params& p, uint32_t m, uint32_t n, float (&d)[4]) {
-    T* at = static_cast<T*>(p.D) + uint64_t(m) * p.ldd + n;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Remote stores of 8 / 16 bytes whose arrival is counted on an mbarrier of the CTA they go to
+__device__ __forceinline__ void st_async(uint32_t at, uint32_t bar, uint32_t a, uint32_t b) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(at), "r"(a), "r"(b), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void st_async(uint32_t at, uint32_t bar, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(a),
+                 "r"(b), "r"(c), "r"(d), "r"(bar)
+                 : "memory");
+}
+// bounded wait that also orders what other CTAs of the cluster wrote
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t polls = 0;; ++polls) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((polls & 63u) == 63u && global_timer_ns() - t0 > limit_ns) return false;
+    }
+}
+
+// `n` finished sums of tokens m0.. for column `col` (a lane's column: a warp writes 32 neighbouring elements of a row of D)
+template <int N, typename T>
+__device__ __forceinline__ void q8_thin_store(const GemmQ8Params& p, uint32_t m0, uint32_t col, const float (&v)[N], const float* sa, float sbn) {
+    if (col >= p.N) return;
+    float d[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[j] = v[j] * (sa[j] * sbn);
     if (p.C != nullptr) {
-        const T* c = static_cast<const T*>(p.C) + uint64_t(m) * p.ldc + n;
+        const T* c = static_cast<const T*>(p.C) + uint64_t(m0) * p.ldc + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < p.N) d[i] = fmaf(p.beta, q8_to_f32(c[i]), d[i]);
+        for (int j = 0; j < N; ++j)
+            if (m0 + j < p.M) d[j] = fmaf(p.beta, q8_to_f32(c[uint64_t(j) * p.ldc]), d[j]);
     }
-    if (p.vec_d && n + 4 <= p.N) {
-        if constexpr (sizeof(T) == 2) {
-            uint2 o;
-            q8_put(reinterpret_cast<T*>(&o) + 0, d[0]);
-            q8_put(reinterpret_cast<T*>(&o) + 1, d[1]);
-            q8_put(reinterpret_cast<T*>(&o) + 2, d[2]);
-            q8_put(reinterpret_cast<T*>(&o) + 3, d[3]);
-            *reinterpret_cast<uint2*>(at) = o;
-        } else {
-            *reinterpret_cast<float4*>(at) = make_float4(d[0], d[1], d[2], d[3]);
-        }
-    } else {
+    T* at = static_cast<T*>(p.D) + uint64_t(m0) * p.ldd + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < p.N) q8_put(at + i, d[i]);
+    for (int j = 0; j < N; ++j)
+        if (m0 + j < p.M) q8_put(at + uint64_t(j) * p.ldd, d[j]);
+}
+
+// Sends this thread's sums (column `n` of the tile, all its tokens) to the ranks that finish them: inbox layout
+// [sender][token / U][128 columns][U], U = 2 or 4 tokens per store.
+template <int BN, int RANKS>
+__device__ __forceinline__ void q8_send(uint32_t taddr, uint32_t inbox, uint32_t bar, uint32_t rank, uint32_t n) {
+    constexpr int TPO = BN / RANKS, U = TPO < 4 ? 2 : 4, CH = BN < 32 ? BN : 32;
+#pragma unroll 1
+    for (int c = 0; c < BN; c += CH) {
+        uint32_t v[32];
+        tmem_ld_32x32(taddr + c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < CH; j += U) {
+            const uint32_t token = c + j, owner = token / TPO, mine = token % TPO;
+            const uint32_t at = map_to_cta(inbox + ((rank * (TPO / U) + mine / U) * 128 + n) * (U * 4), owner), to = map_to_cta(bar, owner);
+            if constexpr (U == 2) st_async(at, to, v[j], v[j + 1]);
+            else st_async(at, to, v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
+    }
+}
+// Adds what has arrived, in rank order, and finishes this rank's tokens.
+template <int BN, int RANKS, typename T>
+__device__ __forceinline__ void q8_finish(const GemmQ8Params& p, const float* inbox, const float* sa, uint32_t rank, uint32_t n, uint32_t tm,
+                                          uint32_t col, float sbn) {
+    constexpr int TPO = BN / RANKS, U = TPO < 4 ? 2 : 4;
+#pragma unroll 1
+    for (int k = 0; k < TPO / U; ++k) {
+        float v[RANKS][U], s[U];
+#pragma unroll
+        for (int r = 0; r < RANKS; ++r) {
+            const float* at = inbox + ((r * (TPO / U) + k) * 128 + n) * U;
+            if constexpr (U == 2) {
+                const float2 f = *reinterpret_cast<const float2*>(at);
+                v[r][0] = f.x; v[r][1] = f.y;
+            } else {
+                const float4 f = *reinterpret_cast<const float4*>(at);
+                v[r][0] = f.x; v[r][1] = f.y; v[r][2] = f.z; v[r][3] = f.w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            s[e] = 0.f;
+#pragma unroll
+            for (int r = 0; r < RANKS; ++r) s[e] += v[r][e];
+        }
+        const uint32_t token = rank * TPO + k * U;
+        if (tm * BN + token >= p.M) break;
+        q8_thin_store<U, T>(p, tm * BN + token, col, s, sa + token, sbn);
     }
 }
 
-// Adds the cluster's partial tiles ([token][128] floats at `partial` in every CTA) in rank order: this CTA's share.
-// All ranks' values of a unit are requested before the first is used: a remote access takes a few hundred cycles.
-template <int RANKS, typename T>
-__device__ __forceinline__ void q8_join(const GemmQ8Params& p, float* partial, const float* sa, uint32_t rank, uint32_t tm0,
-                                        uint32_t tn0, uint32_t tokens) {
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cluster = cg::this_cluster();
-    const float4* from[RANKS];
-#pragma unroll
-    for (int c = 0; c < RANKS; ++c) from[c] = reinterpret_cast<const float4*>(cluster.map_shared_rank(partial, c));
-    for (uint32_t i = rank * blockDim.x + threadIdx.x; i < tokens * 32; i += RANKS * blockDim.x) {
-        const uint32_t j = i >> 5, n = tn0 + (i & 31u) * 4;
-        if (n >= p.N) continue;
-        float4 v[RANKS];
-#pragma unroll
-        for (int c = 0; c < RANKS; ++c) v[c] = from[c][i];
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < RANKS; ++c) {
-            d[0] += v[c].x; d[1] += v[c].y; d[2] += v[c].z; d[3] += v[c].w;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d[e] *= sa[j] * (n + e < p.N ? p.alpha * __ldg(p.sb + n + e) : 0.f);
-        q8_put4<T>(p, tm0 + j, n, d);
-    }
-}
-
-template <int BN, typename T>
+template <int BN, bool SPLIT, typename T>
 __global__ void __launch_bounds__(192)
 gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmQ8Params p) {
-    using Cfg = ThinCfg<BN>;
+    using Cfg = ThinCfg<BN, SPLIT>;
     constexpr int STAGES = Cfg::STAGES;
     extern __shared__ uint8_t q8_smem[];
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
-    const uint32_t full = base + STAGES * Cfg::STAGE, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, slot = accf + 8;
+    const uint32_t full = base + STAGES * Cfg::STAGE, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, inbar = accf + 8, slot = inbar + 8;
     uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
-    float* partial = reinterpret_cast<float*>(smem);                                       // [token][128], reuses the ring
-    float* sa = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE + 256);                // the tile's scales of A
+    float* const sa = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE + 256);          // the tile's scales of A
+    const float* const inbox = sa + BN;                                                    // only with several ranks
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x % p.ranks, tile = blockIdx.x / p.ranks;
@@ -161,16 +206,17 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t n_kb = (p.K + Q8_KB - 1) / Q8_KB;
     const uint32_t kb0 = uint32_t(uint64_t(n_kb) * rank / p.ranks), kb1 = uint32_t(uint64_t(n_kb) * (rank + 1) / p.ranks);
     const uint64_t limit = p.wait_limit_ns;
+    constexpr bool split = SPLIT;
 
     if (threadIdx.x == 0) {
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full + 8 * s, 1);
             mbar_init(empty + 8 * s, 1);
         }
         mbar_init(accf, 1);
+        mbar_init(inbar, 1);
         fence_mbar_init();
+        if (split) mbar_arrive_expect_tx(inbar, Cfg::INBOX);
     }
     if (warp == 1) {
         tmem_alloc<1>(slot, Cfg::TMEM_COLS);
@@ -185,6 +231,7 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    if (split) cluster_arrive();                                      // the inbox barrier is ready
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
 
     bool ok = true;
@@ -214,6 +261,7 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
             uint32_t s = 0, ph = 0;
@@ -234,47 +282,52 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             if (ok) umma_commit<1>(accf);
         }
-    } else {
-        const uint32_t quarter = warp & 3u;
-        const uint32_t n = tn * 128 + quarter * 32 + lane;
-        const float sbn = n < p.N ? p.alpha * __ldg(p.sb + n) : 0.f;
-        if (!mbar_wait_bounded(accf, 0, limit)) {
-            if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-            ok = false;
-        }
+        __syncwarp();
+    }
+    const uint32_t quarter = warp & 3u, n = quarter * 32 + lane, col = tn * 128 + n;       // of an epilogue thread
+    float sbn = 0.f;
+    if (warp >= 2) {
+        sbn = col < p.N ? p.alpha * __ldg(p.sb + col) : 0.f;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
+        if (!ok && lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
         tc_fence_after_sync();
-        const uint32_t taddr = tmem + ((quarter * 32u) << 16);
-        constexpr int CH = BN < 32 ? BN : 32;
+        if (!split && ok) {
+            constexpr int CH = BN < 32 ? BN : 32;
 #pragma unroll 1
-        for (uint32_t c = 0; c < BN && ok; c += CH) {
-            const uint32_t m0 = tm * BN + c;
-            if (m0 >= p.M) break;
-            uint32_t v[32];
-            tmem_ld_32x32(taddr + c, v);
-            tmem_ld_wait();
-            if (p.ranks == 1) {
-                // lane = column: a warp writes 32 neighbouring elements of one row of D at a time
-                float d[CH];
+            for (uint32_t c = 0; c < BN; c += CH) {
+                if (tm * BN + c >= p.M) break;
+                uint32_t v[32];
+                tmem_ld_32x32(tmem + ((quarter * 32u) << 16) + c, v);
+                tmem_ld_wait();
+                float f[CH];
 #pragma unroll
-                for (int j = 0; j < CH; ++j) d[j] = __uint_as_float(v[j]) * (sa[c + j] * sbn);
-                if (n < p.N) {
-                    if (p.C != nullptr) {
-                        const T* cp = static_cast<const T*>(p.C) + uint64_t(m0) * p.ldc + n;
-#pragma unroll
-                        for (int j = 0; j < CH; ++j)
-                            if (m0 + j < p.M) d[j] = fmaf(p.beta, q8_to_f32(cp[uint64_t(j) * p.ldc]), d[j]);
-                    }
-                    T* dp = static_cast<T*>(p.D) + uint64_t(m0) * p.ldd + n;
-#pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        if (m0 + j < p.M) q8_put(dp + uint64_t(j) * p.ldd, d[j]);
-                }
-            } else {
-                // the ring is free: the MMAs that read it have completed
-#pragma unroll
-                for (int j = 0; j < CH; ++j) partial[(c + j) * 128 + quarter * 32 + lane] = __uint_as_float(v[j]);
+                for (int j = 0; j < CH; ++j) f[j] = __uint_as_float(v[j]);
+                q8_thin_store<CH, T>(p, tm * BN + c, col, f, sa + c, sbn);
             }
         }
+    }
+    if (split) {
+        cluster_wait();                                               // every CTA of the cluster is there, its inbox ready
+        if (warp >= 2 && ok) {
+            const uint32_t taddr = tmem + ((quarter * 32u) << 16), in = base + STAGES * Cfg::STAGE + 256 + BN * 4;
+            if (p.ranks == 2) q8_send<BN, 2>(taddr, in, inbar, rank, n);
+            else if (p.ranks == 4) q8_send<BN, 4>(taddr, in, inbar, rank, n);
+            else q8_send<BN, 8>(taddr, in, inbar, rank, n);
+        }
+        __syncwarp();
+        cluster_arrive();                                             // this CTA sends nothing more
+        if (warp >= 2 && ok) {
+            if (!mbar_wait_cluster(inbar, 0, limit)) {
+                if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
+            } else if (p.ranks == 2) {
+                q8_finish<BN, 2, T>(p, inbox, sa, rank, n, tm, col, sbn);
+            } else if (p.ranks == 4) {
+                q8_finish<BN, 4, T>(p, inbox, sa, rank, n, tm, col, sbn);
+            } else {
+                q8_finish<BN, 8, T>(p, inbox, sa, rank, n, tm, col, sbn);
+            }
+        }
+        __syncwarp();
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -282,26 +335,22 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tc_fence_after_sync();
         tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
     }
-    if (p.ranks > 1) {
-        cluster_sync_all();
-        const uint32_t tokens = min(uint32_t(BN), p.M - tm * BN);
-        if (p.ranks == 2) q8_join<2, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
-        else if (p.ranks == 4) q8_join<4, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
-        else q8_join<8, T>(p, partial, sa, rank, tm * BN, tn * 128, tokens);
-        cluster_sync_all();                                           // nobody leaves while its partial tile is being read
-    }
+    if (split) cluster_wait();                                        // nobody is still being sent to by this CTA, nor this one
 }
 
 // =============================================================================================== pair kernel
 struct PairCfg {
     static constexpr uint32_t STAGE = 2 * Q8_TILE;                    // 128 rows of A, 128 rows of B
-    static constexpr int STAGES = 6;
+    static constexpr int STAGES = 5;
     static constexpr int EPI_WARPS = 8;                               // four lane quarters x two column halves
-    static constexpr uint32_t STAGING = EPI_WARPS * 4096;             // per epilogue warp: 32 rows x 128 bytes of D
-    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + 256 /*barriers*/ + 1024 /*scales of B*/;
+    static constexpr int BUFS = 4;                                    // per epilogue warp: boxes of 32 rows x 64 bytes of C and D
+    static constexpr uint32_t BOX = 2048;
+    static constexpr uint32_t STAGING = EPI_WARPS * BUFS * BOX;
+    static constexpr uint32_t BARS = 512;
+    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + BARS + 1024 /*scales of B*/;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 256, 256);
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static_assert(16 * STAGES + 32 + 8 <= 256, "barrier area");
+    static_assert(16 * STAGES + 32 + 8 * EPI_WARPS * BUFS + 8 <= BARS, "barrier area");
     static_assert(SMEM_BYTES <= 227 * 1024, "one CTA's shared memory");
 };
 
@@ -313,71 +362,19 @@ __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p
     tn = r / rows;
 }
 
-// 32 columns col0.. of one row of C, if there are that many: a lane reads whole 128-byte lines (64 for fp16)
-template <typename T>
-__device__ __forceinline__ void q8_load_c(const GemmQ8Params& p, uint32_t row, uint32_t col0, uint4 (&c)[sizeof(T) * 2]) {
-    if (row >= p.M || col0 >= p.N) return;
-    const T* at = static_cast<const T*>(p.C) + uint64_t(row) * p.ldc + col0;
-    if (p.vec_c && col0 + 32 <= p.N) {
-#pragma unroll
-        for (int u = 0; u < int(sizeof(T)) * 2; ++u) c[u] = reinterpret_cast<const uint4*>(at)[u];
-    } else {
-        T* e = reinterpret_cast<T*>(&c);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) e[i] = col0 + i < p.N ? at[i] : T(0.f);
-    }
-}
-
-// 32 finished columns col0.. of `row`, scaled by sa * sb[0..31], (+ beta * C), to the staging row (16-byte units unit0..,
-// swizzled) or to D
-template <typename T>
-__device__ __forceinline__ void q8_store_chunk(const GemmQ8Params& p, uint32_t row, uint32_t col0, const uint32_t (&v)[32], float sa,
-                                               const float* sb, const uint4 (&c)[sizeof(T) * 2], uint32_t stage_row, uint32_t unit0) {
-    constexpr int PER = 16 / sizeof(T);                               // elements per 16-byte unit
-    const uint32_t ncols = min(32u, p.N - col0), sw = (stage_row >> 7) & 7u;
-    T* drow = static_cast<T*>(p.D) + uint64_t(row) * p.ldd + col0;
-#pragma unroll
-    for (int u = 0; u < 32 / PER; ++u) {
-        float d[PER];
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            const float4 b = reinterpret_cast<const float4*>(sb)[(u * PER + i) / 4];
-            d[i] = __uint_as_float(v[u * PER + i]) * (sa * b.x);
-            d[i + 1] = __uint_as_float(v[u * PER + i + 1]) * (sa * b.y);
-            d[i + 2] = __uint_as_float(v[u * PER + i + 2]) * (sa * b.z);
-            d[i + 3] = __uint_as_float(v[u * PER + i + 3]) * (sa * b.w);
-        }
-        if (p.C != nullptr) {
-            const T* e = reinterpret_cast<const T*>(&c[u]);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) d[i] = fmaf(p.beta, q8_to_f32(e[i]), d[i]);
-        }
-        uint4 o;
-        T* e = reinterpret_cast<T*>(&o);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) q8_put(e + i, d[i]);
-        if (stage_row != 0) {
-            st_shared_v4(stage_row + (((unit0 + u) ^ sw) << 4), o.x, o.y, o.z, o.w);
-        } else if (row < p.M) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (u * PER + i < ncols) drow[u * PER + i] = e[i];
-        }
-    }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(PairCfg::THREADS, 1)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmD, const GemmQ8Params p) {
-    constexpr int STAGES = PairCfg::STAGES;
+                    const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmC, const GemmQ8Params p) {
+    using Cfg = PairCfg;
+    constexpr int STAGES = Cfg::STAGES;
     extern __shared__ uint8_t q8_smem[];
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
-    const uint32_t staging = base + STAGES * PairCfg::STAGE;
-    const uint32_t full = staging + PairCfg::STAGING, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, acce = accf + 16;
-    const uint32_t slot = acce + 16;
+    const uint32_t staging = base + STAGES * Cfg::STAGE;
+    const uint32_t full = staging + Cfg::STAGING, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, acce = accf + 16;
+    const uint32_t cbar0 = acce + 16, slot = cbar0 + 8 * Cfg::EPI_WARPS * Cfg::BUFS;
     uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
-    float* const sb_tile = reinterpret_cast<float*>(smem + (full + 256 - base));       // the tile's 256 scales of B
+    float* const sb_tile = reinterpret_cast<float*>(smem + (full + Cfg::BARS - base));     // the tile's scales of B
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = cluster_ctarank();
@@ -393,8 +390,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(accf + 8 * a, 1);
-            mbar_init(acce + 8 * a, 2 * PairCfg::EPI_WARPS);          // the epilogue warps of both CTAs
+            mbar_init(acce + 8 * a, 2 * Cfg::EPI_WARPS);              // the epilogue warps of both CTAs
         }
+        for (int w = 0; w < Cfg::EPI_WARPS * Cfg::BUFS; ++w) mbar_init(cbar0 + 8 * w, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -411,8 +409,6 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
         if (lane == 0) {
-            tma_prefetch_desc(&tmA);
-            tma_prefetch_desc(&tmB);
             const uint32_t full0 = map_to_cta(full, 0);
             uint32_t s = 0, ph = 0;
             bool ok = true;
@@ -426,8 +422,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         ok = false;
                         break;
                     }
-                    const uint32_t stage = base + s * PairCfg::STAGE, fb = full0 + 8 * s;
-                    if (leader) mbar_arrive_expect_tx(full + 8 * s, 2 * PairCfg::STAGE);
+                    const uint32_t stage = base + s * Cfg::STAGE, fb = full0 + 8 * s;
+                    if (leader) mbar_arrive_expect_tx(full + 8 * s, 2 * Cfg::STAGE);
                     tma_load_2d_pair(stage, &tmA, fb, int32_t(kb * Q8_KB), arow);
                     tma_load_2d_pair(stage + Q8_TILE, &tmB, fb, int32_t(kb * Q8_KB), brow);
                     if (++s == STAGES) { s = 0; ph ^= 1u; }
@@ -437,10 +433,17 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             for (int i = 0; i < STAGES && ok; ++i) {
                 if (!mbar_wait_bounded(empty + 8 * s, ph ^ 1u, limit)) {
                     q8_report(p, Q8_TIMEOUT_TAIL);
+                    ok = false;
                     break;
                 }
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
             }
+            // the MMA side is stuck: at least both CTAs' copies (counted on the leader's barriers) have to land
+            if (!ok && leader)
+                for (int i = 0; i < STAGES; ++i) {
+                    (void)mbar_wait_bounded(full + 8 * s, ph ^ 1u, limit / 8);
+                    if (++s == STAGES) { s = 0; ph ^= 1u; }
+                }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
@@ -449,7 +452,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             uint32_t s = 0, ph = 0, it = 0;
             bool ok = true;
             for (uint32_t t = worker; t < n_tiles && ok; t += workers, ++it) {
-                const uint32_t a = it & 1u, aph = (it >> 1) & 1u;
+                const uint32_t a = it & 1u, aph = (it >> 1) & 1u;     // tiles alternate between two accumulators
                 if (!mbar_wait_bounded(acce + 8 * a, aph ^ 1u, limit)) {
                     q8_report(p, Q8_TIMEOUT_MMA_ACC);
                     ok = false;
@@ -463,11 +466,11 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         break;
                     }
                     tc_fence_after_sync();
-                    const uint32_t stage = base + s * PairCfg::STAGE;
+                    const uint32_t stage = base + s * Cfg::STAGE;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_q8<2>(tmem + a * 256, smem_desc_at(Q8_DESC, stage + k * 32),
-                                   smem_desc_at(Q8_DESC, stage + Q8_TILE + k * 32), PairCfg::IDESC, (kb | uint32_t(k)) ? 1u : 0u);
+                        umma_q8<2>(tmem + a * 256, smem_desc_at(Q8_DESC, stage + k * 32), smem_desc_at(Q8_DESC, stage + Q8_TILE + k * 32),
+                                   Cfg::IDESC, (kb | uint32_t(k)) ? 1u : 0u);
                     umma_commit<2>(empty + 8 * s);
                     umma_commit<2>(peer_empty + 8 * s);
                     if (++s == STAGES) { s = 0; ph ^= 1u; }
@@ -486,66 +489,145 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
     } else {
         // ------------------------------------------------------------------ epilogue
-        const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;  // TMEM lanes [32 quarter, +32), columns [128 half, +128)
+        // Warp (quarter, half): TMEM lanes [32 quarter, +32), columns [128 half, +128), 64 bytes of D
+        // per row at a time.  A box of C arrives by TMA in one of the warp's four buffers, is turned into D in place and
+        // leaves by TMA; the boxes two ahead are asked for meanwhile, those of a tile's start while it is multiplied.
+        constexpr uint32_t CW = 64 / sizeof(T);                       // columns of a box
+        constexpr uint32_t BOXES = 128 / CW;                          // of a tile
+        constexpr int PER = 16 / sizeof(T);                           // elements of a 16-byte unit
+        const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;
         const uint32_t acce0 = map_to_cta(acce, 0);
-        const uint32_t stage_warp = staging + (warp - 2u) * 4096u;
-        const uint32_t stage_row = p.d_tma ? stage_warp + lane * 128u : 0u;
-        constexpr uint32_t BOX = 128 / sizeof(T);                     // columns of one staged box
-        constexpr uint32_t SUB = BOX / 32;                            // 32-column chunks per box
+        const uint32_t bufs = staging + (warp - 2u) * Cfg::BUFS * Cfg::BOX, cbar = cbar0 + 8 * (warp - 2u) * Cfg::BUFS;
+        const uint32_t sw = (lane >> 1) & 3u;                         // 64-byte swizzle: unit ^ (row / 2) % 4
         // TMA clips a column edge in 16-byte units: a box that crosses an edge N which is not 16-byte aligned is
         // written by predicated per-thread stores
         const bool ragged = ((p.N * uint32_t(sizeof(T))) & 15u) != 0u;
-        uint32_t it = 0;
+        uint32_t it = 0, q = 0, cphase = 0, asked = 0;                // q: boxes so far; a phase bit, and whether C is on its way, per buffer
         bool ok = true;
         for (uint32_t t = worker; t < n_tiles; t += workers, ++it) {
             uint32_t tm, tn;
             q8_tile_coords(t, p, tm, tn);
-            const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane, colbase = tn * 256 + half * 128;
+            const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane;
+            auto box_col = [&](uint32_t i) { return tn * 256 + half * 128 + i * CW; };
+            auto boxed = [&](uint32_t col) { return p.d_tma && col < p.N && warp_row0 < p.M && !(ragged && col + CW > p.N); };
+            auto fetch_c = [&](uint32_t i) {                          // box i of this tile into buffer (q + i) % 4
+                if (i < BOXES && p.c_tma && boxed(box_col(i))) {
+                    const uint32_t b = (q + i) % Cfg::BUFS;
+                    asked |= 1u << b;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(cbar + 8 * b, Cfg::BOX);
+                        tma_load_2d(bufs + b * Cfg::BOX, &tmC, cbar + 8 * b, int32_t(box_col(i)), int32_t(warp_row0));
+                    }
+                }
+            };
             const float sa = row < p.M ? p.alpha * p.sa[row] : 0.f;
             // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more, and C
             const uint32_t sb_col = tn * 256 + threadIdx.x - 64;
             const float sb_mine = sb_col < p.N ? __ldg(p.sb + sb_col) : 0.f;
-            uint4 cbuf[2][sizeof(T) * 2];
-            if (p.C != nullptr) q8_load_c<T>(p, row, colbase, cbuf[0]);
+            if (ok && p.c_tma) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");     // buffers q, q + 1 are free
+                fetch_c(0);
+                fetch_c(1);
+            }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             sb_tile[threadIdx.x - 64] = sb_mine;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const uint32_t a = it & 1u, aph = (it >> 1) & 1u;
-            if (ok && !mbar_wait_bounded(accf + 8 * a, aph, limit)) {
+            if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(accf + 8 * a, aph, limit))) {
                 if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-                ok = false;                                           // keeps to the barriers above, touches nothing more
+                ok = false;                                       // keeps to the barriers above, touches nothing more
             }
             tc_fence_after_sync();
             const uint32_t taddr = tmem + a * 256 + half * 128 + ((quarter * 32u) << 16);
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-                const uint32_t col0 = colbase + c * 32;
-                if (!ok || col0 >= p.N) break;
-                if (p.C != nullptr && c < 3) q8_load_c<T>(p, row, col0 + 32, cbuf[(c + 1) & 1]);
+#pragma unroll 1
+            for (uint32_t c = 0; c < 4 && ok; ++c) {              // 32 columns at a time: one box of fp16, two of fp32
+                if (tn * 256 + half * 128 + c * 32 >= p.N) {
+                    for (uint32_t k = 0; k < 32 / CW; ++k) {      // boxes that do not exist keep their place
+                        if (lane == 0) bulk_commit_group();
+                    }
+                    continue;
+                }
                 uint32_t v[32];
                 tmem_ld_32x32(taddr + c * 32, v);
                 tmem_ld_wait();
-                const uint32_t sub = c & (SUB - 1), box0 = col0 - sub * 32;
-                const bool boxed = p.d_tma && !(ragged && box0 + BOX > p.N);
-                if (boxed && sub == 0) {
-                    if (lane == 0) bulk_wait_read_all();              // the previous box has left the staging tile
-                    __syncwarp();
-                }
-                q8_store_chunk<T>(p, row, col0, v, sa, sb_tile + half * 128 + c * 32, cbuf[c & 1], boxed ? stage_row : 0u, sub * (8 / SUB));
-                if (boxed && (sub == SUB - 1 || col0 + 32 >= p.N)) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0 && warp_row0 < p.M) {
-                        tma_store_2d(&tmD, stage_warp, int32_t(box0), int32_t(warp_row0));
-                        bulk_commit_group();
+#pragma unroll
+                for (uint32_t k = 0; k < 32 / CW; ++k) {
+                    const uint32_t i = c * (32 / CW) + k, col = box_col(i), b = (q + i) % Cfg::BUFS;
+                    const bool box = boxed(col);
+                    // the store that left from this buffer four boxes ago, and the one two ahead's, have been read
+                    if (lane == 0) {
+                        if (p.c_tma) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        else asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
                     }
+                    __syncwarp();
+                    fetch_c(i + 2);
+                    const bool c_box = box && p.c_tma;
+                    if (c_box) {
+                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(cbar + 8 * b, (cphase >> b) & 1u, limit))) {
+                            if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
+                            ok = false;
+                        }
+                        cphase ^= 1u << b;
+                        asked ^= 1u << b;
+                    }
+                    const uint32_t at = bufs + b * Cfg::BOX + lane * 64;
+                    const float* sbp = sb_tile + half * 128 + c * 32 + k * CW;
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        float d[PER];
+#pragma unroll
+                        for (int e = 0; e < PER; e += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(sbp + u * PER + e);
+                            d[e] = __uint_as_float(v[k * CW + u * PER + e]) * (sa * f.x);
+                            d[e + 1] = __uint_as_float(v[k * CW + u * PER + e + 1]) * (sa * f.y);
+                            d[e + 2] = __uint_as_float(v[k * CW + u * PER + e + 2]) * (sa * f.z);
+                            d[e + 3] = __uint_as_float(v[k * CW + u * PER + e + 3]) * (sa * f.w);
+                        }
+                        const uint32_t unit = at + ((u ^ sw) << 4);
+                        const uint32_t left = col + u * PER < p.N ? p.N - col - u * PER : 0u;      // columns from here on
+                        if (p.C != nullptr) {
+                            if (c_box) {
+                                const uint4 w = ld_shared_v4(unit);
+                                const T* cp = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                                for (int e = 0; e < PER; ++e) d[e] = fmaf(p.beta, q8_to_f32(cp[e]), d[e]);
+                            } else if (row < p.M) {
+                                const T* cp = static_cast<const T*>(p.C) + uint64_t(row) * p.ldc + col + u * PER;
+#pragma unroll
+                                for (int e = 0; e < PER; ++e)
+                                    if (uint32_t(e) < left) d[e] = fmaf(p.beta, q8_to_f32(cp[e]), d[e]);
+                            }
+                        }
+                        uint4 o;
+                        T* op = reinterpret_cast<T*>(&o);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) q8_put(op + e, d[e]);
+                        if (box) {
+                            st_shared_v4(unit, o.x, o.y, o.z, o.w);
+                        } else if (row < p.M) {
+                            T* dp = static_cast<T*>(p.D) + uint64_t(row) * p.ldd + col + u * PER;
+#pragma unroll
+                            for (int e = 0; e < PER; ++e)
+                                if (uint32_t(e) < left) dp[e] = op[e];
+                        }
+                    }
+                    if (box) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tma_store_2d(&tmD, bufs + b * Cfg::BOX, int32_t(col), int32_t(warp_row0));
+                    }
+                    if (lane == 0) bulk_commit_group();           // one group per box, stored or not
                 }
             }
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0 && ok) mbar_arrive_cluster(acce0 + 8 * a);
+            q += BOXES;
         }
-        if (lane == 0 && p.d_tma) bulk_wait_all();
+        if (lane == 0) bulk_wait_all();
+        if (!ok)                                                      // copies still on their way have to land first
+            for (uint32_t b = 0; b < Cfg::BUFS; ++b)
+                if ((asked >> b) & 1u) (void)mbar_wait_bounded(cbar + 8 * b, (cphase >> b) & 1u, limit);
     }
 
     tc_fence_before_sync();

@@ -235,8 +235,8 @@ DECXB200_API int decxb200_cast2d(int kind, void* stream, uint32_t rows, uint32_t
  *   with D's pitch.  alpha, beta: host pointers, NULL means 1 / 0; C is not read when beta == 0.
  *   Sums are fp32; an fp16 D is rounded once.  tcgen05 kind::f8f6f4; one launch, no workspace, the same result every
  *   time.  lda, ldb: multiples of 16, bases 16-byte aligned.  status as for decxb200_gemm.  Asynchronous on `stream`.
- *   tile: DECXB200_TILE_AUTO, or one of the two kernels (tests and measurements): THIN cuts K over a cluster of CTAs
- *   and is made for few rows of A, PAIR works on 256 x 256 tiles.
+ *   tile: DECXB200_TILE_AUTO, or one of the kernels (tests and measurements): THIN cuts K over a cluster of CTAs and is
+ *   made for few rows of A, PAIR works on 256 x 256 tiles.
  */
 #define DECXB200_TILE_Q8_THIN 1
 #define DECXB200_TILE_Q8_PAIR 2
