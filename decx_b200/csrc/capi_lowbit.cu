@@ -215,6 +215,46 @@ int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) 
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit GEMM
+// How many clusters of `size` CTAs of a kernel the GPU holds at once (asked once per kernel and size)
+template <typename K>
+int clusters_at_once(K kern, unsigned threads, unsigned smem, unsigned size, std::atomic<int>& known) {
+    int n = known.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr[2];
+        cluster_config(cfg, attr, size, threads, smem, size, nullptr);
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) n = -1;
+        known.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// How many CTAs cut a tile's K in the thin kernel: as many as are on the GPU at once (up to 64 tokens, whose CTAs are short
+// and share their SMs, a quarter more: 64 x 4096 x 16384 takes 17 us so and 20 us with half as many), at least two stages
+// each
+template <int BN, typename T>
+uint32_t q8_thin_ranks(uint64_t tiles, uint32_t n_kb) {
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> held[4];
+    auto kern = gemm_q8_thin_kernel<BN, true, T>;
+    using Cfg = ThinCfg<BN, true>;
+    if (allow_smem(kern, Cfg::SMEM_BYTES, done) != 0) return 1;
+    uint32_t ranks = 1;
+    for (int i = 1; i < 4; ++i)
+        if (n_kb >= (2u << i) && int64_t(tiles) * (BN < 128 ? 4 : 5) <= 5 * int64_t(clusters_at_once(kern, 192, Cfg::SMEM_BYTES, 1u << i, held[i])))
+            ranks = 1u << i;
+    return ranks;
+}
+// Whether two pairs share a tile's K in the pair kernel: if all tiles are on the GPU at once
+template <typename T>
+bool q8_pair_split(uint64_t tiles, uint32_t n_kb) {
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> held;
+    auto kern = gemm_q8_pair_kernel<true, T>;
+    if (n_kb < 8 || tiles > 37 || allow_smem(kern, PairCfg::SMEM_BYTES, done) != 0) return false;
+    return int64_t(tiles) <= clusters_at_once(kern, PairCfg::THREADS, PairCfg::SMEM_BYTES, 4, held);
+}
+
 template <int BN, bool SPLIT, typename T>
 int launch_q8_thin(cudaStream_t s, const GemmQ8Params& p, const CUtensorMap& ma, const CUtensorMap& mb) {
     using Cfg = ThinCfg<BN, SPLIT>;
@@ -237,10 +277,7 @@ int run_q8_thin(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, con
     p.tiles_n = (p.N + 127) / 128;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     const uint32_t n_kb = (p.K + Q8_KB - 1) / Q8_KB;
-    // cut K until the GPU is full (two CTAs per SM; BN 128: one), at least two stages each
-    const uint64_t room = BN == 128 ? 148 : 296;
-    p.ranks = 1;
-    while (p.ranks < 8 && tiles * p.ranks * 2 <= room && n_kb >= p.ranks * 2 * 2) p.ranks *= 2;
+    p.ranks = q8_thin_ranks<BN, T>(tiles, n_kb);
     return p.ranks > 1 ? launch_q8_thin<BN, true, T>(s, p, ma, mb) : launch_q8_thin<BN, false, T>(s, p, ma, mb);
 }
 
@@ -259,14 +296,16 @@ int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
     if (p.d_tma && p.C != nullptr && aligned16(p.C) && (p.ldc * e) % 16 == 0 &&
         dxb_host::tensor_map_2d(&mc, int(e), p.C, p.M, p.N, p.ldc, uint32_t(64 / e), 32) == 0)
         p.c_tma = 1;
-    auto kern = gemm_q8_pair_kernel<T>;
-    static std::atomic<uint64_t> done{0};
-    if ((rc = allow_smem(kern, Cfg::SMEM_BYTES, done)) != 0) return rc;
     p.tiles_m = uint32_t((uint64_t(p.M) + 255) / 256);
     p.tiles_n = uint32_t((uint64_t(p.N) + 255) / 256);
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     if (tiles > 0x7fffffffull) return DECXB200_ETOOLARGE;
     p.group_m = p.tiles_m < 8 ? p.tiles_m : 8;
+    if (q8_pair_split<T>(tiles, (p.K + Q8_KB - 1) / Q8_KB))
+        return launch_cluster(gemm_q8_pair_kernel<true, T>, unsigned(4 * tiles), Cfg::THREADS, Cfg::SMEM_BYTES, 4, s, ma, mb, md, mc, p);
+    static std::atomic<uint64_t> done{0};
+    auto kern = gemm_q8_pair_kernel<false, T>;
+    if ((rc = allow_smem(kern, Cfg::SMEM_BYTES, done)) != 0) return rc;
     uint64_t pairs = uint64_t(sm_count()) / 2;
     if (pairs > tiles) pairs = tiles;
     if (pairs == 0) pairs = 1;
@@ -276,8 +315,18 @@ int launch_q8_pair(cudaStream_t s, GemmQ8Params p, const void* A, uint64_t lda, 
 template <typename T>
 int run_gemm_q8(cudaStream_t s, const GemmQ8Params& p, const void* A, uint64_t lda, const void* B, uint64_t ldb, int tile) {
     if (tile == DECXB200_TILE_AUTO) {
-        const uint64_t tiles = (uint64_t(p.M) + 255) / 256 * ((uint64_t(p.N) + 255) / 256);
-        tile = p.M > 128 && tiles >= 48 ? DECXB200_TILE_Q8_PAIR : DECXB200_TILE_Q8_THIN;
+        // Clocks of either kernel: turns on the SMs x 128s of K (700 each, measured, for a 256 x 256 tile of a pair as for a
+        // 128 x 128 tile of one SM), and what comes after the sums, longer when they are joined.
+        tile = DECXB200_TILE_Q8_THIN;
+        if (p.M > 128) {
+            const uint64_t n_kb = (uint64_t(p.K) + Q8_KB - 1) / Q8_KB;
+            const uint64_t tiles = (uint64_t(p.M) + 255) / 256 * ((uint64_t(p.N) + 255) / 256);
+            const uint64_t thin_tiles = (uint64_t(p.M) + 127) / 128 * ((uint64_t(p.N) + 127) / 128);
+            const uint64_t r = q8_pair_split<T>(tiles, uint32_t(n_kb)) ? 2 : 1, tr = q8_thin_ranks<128, T>(thin_tiles, uint32_t(n_kb));
+            const uint64_t pair = (tiles * r + 73) / 74 * (n_kb / r) * 700 + (r > 1 ? 12000 : 5000);
+            const uint64_t thin = (thin_tiles * tr + 147) / 148 * (n_kb / tr) * 700 + (tr > 1 ? 8500 : 3000);
+            if (pair < thin) tile = DECXB200_TILE_Q8_PAIR;
+        }
     }
     if (tile == DECXB200_TILE_Q8_PAIR) return launch_q8_pair<T>(s, p, A, lda, B, ldb);
     if (p.M <= 16) return run_q8_thin<16, T>(s, p, A, lda, B, ldb);

@@ -350,7 +350,9 @@ struct PairCfg {
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + STAGING + 1024 /*alignment slack*/ + BARS + 1024 /*scales of B*/;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 256, 256);
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static_assert(16 * STAGES + 32 + 8 * EPI_WARPS * BUFS + 8 <= BARS, "barrier area");
+    static constexpr uint32_t INBOX = 128 * 128 * 4;                  // SPLIT: the other pair's sums of this CTA's columns, in the
+    static_assert(INBOX <= STAGES * STAGE, "inbox");                  // ring's place
+    static_assert(16 * STAGES + 32 + 8 * EPI_WARPS * BUFS + 16 <= BARS, "barrier area");
     static_assert(SMEM_BYTES <= 227 * 1024, "one CTA's shared memory");
 };
 
@@ -362,7 +364,10 @@ __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p
     tn = r / rows;
 }
 
-template <typename T>
+// SPLIT: two pairs (a cluster of four CTAs) share a tile, each half of K.  Pair r finishes columns [128 r, +128): the CTAs that
+// hold the same rows send each other the other half, as the thin kernel does, and into the ring, which is free once
+// both pairs' MMAs are done.
+template <bool SPLIT, typename T>
 __global__ void __launch_bounds__(PairCfg::THREADS, 1)
 gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmC, const GemmQ8Params p) {
@@ -372,15 +377,18 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t base = (smem_u32(q8_smem) + 1023u) & ~1023u;
     const uint32_t staging = base + STAGES * Cfg::STAGE;
     const uint32_t full = staging + Cfg::STAGING, empty = full + 8 * STAGES, accf = empty + 8 * STAGES, acce = accf + 16;
-    const uint32_t cbar0 = acce + 16, slot = cbar0 + 8 * Cfg::EPI_WARPS * Cfg::BUFS;
+    const uint32_t cbar0 = acce + 16, inbar = cbar0 + 8 * Cfg::EPI_WARPS * Cfg::BUFS, slot = inbar + 8;
     uint8_t* const smem = q8_smem + (base - smem_u32(q8_smem));
     float* const sb_tile = reinterpret_cast<float*>(smem + (full + Cfg::BARS - base));     // the tile's scales of B
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t cta = cluster_ctarank();
+    const uint32_t in_cluster = cluster_ctarank(), cta = in_cluster & 1u, rank = SPLIT ? in_cluster >> 1 : 0u;
+    const uint32_t lead = in_cluster & ~1u, peer = in_cluster | 1u;   // this pair's CTAs within the cluster
     const bool leader = cta == 0;
-    const uint32_t workers = gridDim.x / 2, worker = blockIdx.x / 2;
-    const uint32_t n_tiles = p.tiles_m * p.tiles_n, n_kb = (p.K + Q8_KB - 1) / Q8_KB;
+    constexpr uint32_t ranks = SPLIT ? 2 : 1;
+    const uint32_t workers = gridDim.x / (2 * ranks), worker = blockIdx.x / (2 * ranks);
+    const uint32_t n_tiles = p.tiles_m * p.tiles_n, all_kb = (p.K + Q8_KB - 1) / Q8_KB;
+    const uint32_t kb0 = uint32_t(uint64_t(all_kb) * rank / ranks), n_kb = uint32_t(uint64_t(all_kb) * (rank + 1) / ranks) - kb0;
     const uint64_t limit = p.wait_limit_ns;
 
     if (threadIdx.x == 0) {
@@ -393,7 +401,9 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             mbar_init(acce + 8 * a, 2 * Cfg::EPI_WARPS);              // the epilogue warps of both CTAs
         }
         for (int w = 0; w < Cfg::EPI_WARPS * Cfg::BUFS; ++w) mbar_init(cbar0 + 8 * w, 1);
+        mbar_init(inbar, 1);
         fence_mbar_init();
+        if (SPLIT) mbar_arrive_expect_tx(inbar, Cfg::INBOX);
     }
     if (warp == 1) {
         tmem_alloc<2>(slot, 512);
@@ -409,7 +419,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
         if (lane == 0) {
-            const uint32_t full0 = map_to_cta(full, 0);
+            const uint32_t full0 = map_to_cta(full, lead);
             uint32_t s = 0, ph = 0;
             bool ok = true;
             for (uint32_t t = worker; t < n_tiles && ok; t += workers) {
@@ -424,8 +434,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                     const uint32_t stage = base + s * Cfg::STAGE, fb = full0 + 8 * s;
                     if (leader) mbar_arrive_expect_tx(full + 8 * s, 2 * Cfg::STAGE);
-                    tma_load_2d_pair(stage, &tmA, fb, int32_t(kb * Q8_KB), arow);
-                    tma_load_2d_pair(stage + Q8_TILE, &tmB, fb, int32_t(kb * Q8_KB), brow);
+                    tma_load_2d_pair(stage, &tmA, fb, int32_t((kb0 + kb) * Q8_KB), arow);
+                    tma_load_2d_pair(stage + Q8_TILE, &tmB, fb, int32_t((kb0 + kb) * Q8_KB), brow);
                     if (++s == STAGES) { s = 0; ph ^= 1u; }
                 }
             }
@@ -448,7 +458,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
         if (leader && lane == 0) {
-            const uint32_t peer_empty = map_to_cta(empty, 1), peer_accf = map_to_cta(accf, 1);
+            const uint32_t peer_empty = map_to_cta(empty, peer), peer_accf = map_to_cta(accf, peer);
             uint32_t s = 0, ph = 0, it = 0;
             bool ok = true;
             for (uint32_t t = worker; t < n_tiles && ok; t += workers, ++it) {
@@ -480,12 +490,21 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     umma_commit<2>(peer_accf + 8 * a);
                 }
             }
-            for (int i = 0; i < 2 && ok; ++i, ++it) {                 // both accumulators drained by both CTAs
+            // both accumulators drained by both CTAs (SPLIT: the barrier at the end sees to that; the epilogue waits for this
+            // warp first)
+            for (int i = 0; i < 2 && ok && !SPLIT; ++i, ++it) {
                 if (!mbar_wait_bounded(acce + 8 * (it & 1u), ((it >> 1) & 1u) ^ 1u, limit)) {
                     q8_report(p, Q8_TIMEOUT_TAIL);
                     break;
                 }
             }
+        }
+    }
+    if (warp < 2) {
+        __syncwarp();
+        if (SPLIT) {                                                  // the epilogue's handshake needs all threads
+            cluster_arrive();
+            cluster_wait();
         }
     } else {
         // ------------------------------------------------------------------ epilogue
@@ -493,10 +512,10 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         // per row at a time.  A box of C arrives by TMA in one of the warp's four buffers, is turned into D in place and
         // leaves by TMA; the boxes two ahead are asked for meanwhile, those of a tile's start while it is multiplied.
         constexpr uint32_t CW = 64 / sizeof(T);                       // columns of a box
-        constexpr uint32_t BOXES = 128 / CW;                          // of a tile
+        constexpr uint32_t share = 128 / ranks, BOXES = share / CW;   // columns this warp finishes of a tile, in so many boxes
         constexpr int PER = 16 / sizeof(T);                           // elements of a 16-byte unit
         const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;
-        const uint32_t acce0 = map_to_cta(acce, 0);
+        const uint32_t acce0 = map_to_cta(acce, lead);
         const uint32_t bufs = staging + (warp - 2u) * Cfg::BUFS * Cfg::BOX, cbar = cbar0 + 8 * (warp - 2u) * Cfg::BUFS;
         const uint32_t sw = (lane >> 1) & 3u;                         // 64-byte swizzle: unit ^ (row / 2) % 4
         // TMA clips a column edge in 16-byte units: a box that crosses an edge N which is not 16-byte aligned is
@@ -508,7 +527,8 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             uint32_t tm, tn;
             q8_tile_coords(t, p, tm, tn);
             const uint32_t warp_row0 = (tm * 2 + cta) * 128 + quarter * 32, row = warp_row0 + lane;
-            auto box_col = [&](uint32_t i) { return tn * 256 + half * 128 + i * CW; };
+            const uint32_t col_in_tile = SPLIT ? rank * 128 + half * share : half * 128;
+            auto box_col = [&](uint32_t i) { return tn * 256 + col_in_tile + i * CW; };
             auto boxed = [&](uint32_t col) { return p.d_tma && col < p.N && warp_row0 < p.M && !(ragged && col + CW > p.N); };
             auto fetch_c = [&](uint32_t i) {                          // box i of this tile into buffer (q + i) % 4
                 if (i < BOXES && p.c_tma && boxed(box_col(i))) {
@@ -538,18 +558,51 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 ok = false;                                       // keeps to the barriers above, touches nothing more
             }
             tc_fence_after_sync();
-            const uint32_t taddr = tmem + a * 256 + half * 128 + ((quarter * 32u) << 16);
+            if constexpr (SPLIT) {
+                __syncwarp();
+                cluster_arrive();                                     // this pair's MMAs have read the ring
+                cluster_wait();                                       // the other pair's have, too
+                if (ok) {
+                    // this warp's 64 of the columns that the other pair finishes: inbox layout [column / 4][128 rows][4]
+                    const uint32_t other = (rank ^ 1u) * 2 + cta, to = map_to_cta(inbar, other);
+                    const uint32_t at = map_to_cta(base + (half * share / 4 * 128 + quarter * 32 + lane) * 16, other);
+                    const uint32_t src = tmem + (rank ^ 1u) * 128 + half * share + ((quarter * 32u) << 16);
+#pragma unroll
+                    for (uint32_t c = 0; c < share / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld_32x32(src + c * 32, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (uint32_t j = 0; j < 32; j += 4) st_async(at + (c * 32 + j) / 4 * 2048, to, v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    }
+                    if (!__all_sync(0xffffffffu, mbar_wait_cluster(inbar, 0, limit))) {
+                        if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
+                        ok = false;
+                    }
+                }
+            }
 #pragma unroll 1
-            for (uint32_t c = 0; c < 4 && ok; ++c) {              // 32 columns at a time: one box of fp16, two of fp32
-                if (tn * 256 + half * 128 + c * 32 >= p.N) {
+            for (uint32_t c = 0; c < share / 32 && ok; ++c) {     // 32 columns at a time: one box of fp16, two of fp32
+                if (box_col(c * (32 / CW)) >= p.N) {
                     for (uint32_t k = 0; k < 32 / CW; ++k) {      // boxes that do not exist keep their place
                         if (lane == 0) bulk_commit_group();
                     }
                     continue;
                 }
                 uint32_t v[32];
-                tmem_ld_32x32(taddr + c * 32, v);
+                tmem_ld_32x32(tmem + a * 256 + col_in_tile + c * 32 + ((quarter * 32u) << 16), v);
                 tmem_ld_wait();
+                if constexpr (SPLIT) {                                // and what has arrived (two terms: the order does not matter)
+                    const float4* in = reinterpret_cast<const float4*>(smem) + (half * share + c * 32) / 4 * 128 + quarter * 32 + lane;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        const float4 g = in[j * 128];
+                        v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + g.x);
+                        v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + g.y);
+                        v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + g.z);
+                        v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + g.w);
+                    }
+                }
 #pragma unroll
                 for (uint32_t k = 0; k < 32 / CW; ++k) {
                     const uint32_t i = c * (32 / CW) + k, col = box_col(i), b = (q + i) % Cfg::BUFS;
@@ -571,7 +624,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         asked ^= 1u << b;
                     }
                     const uint32_t at = bufs + b * Cfg::BOX + lane * 64;
-                    const float* sbp = sb_tile + half * 128 + c * 32 + k * CW;
+                    const float* sbp = sb_tile + col_in_tile + c * 32 + k * CW;
 #pragma unroll
                     for (uint32_t u = 0; u < 4; ++u) {
                         float d[PER];

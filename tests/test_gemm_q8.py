@@ -12,7 +12,8 @@ THIN, PAIR = 1, 2
 # stages than the ring has, of a short last stage, long enough to be cut eight ways; several rounds of tiles
 SHAPES = [(1, 1, 1), (1, 128, 128), (7, 40, 16), (16, 256, 300), (17, 129, 1000), (32, 1000, 4096), (33, 64, 130), (64, 513, 2047),
           (65, 300, 513), (128, 128, 8192), (129, 257, 1025), (256, 256, 256), (300, 700, 777), (513, 1030, 384), (1, 5000, 520),
-          (2600, 2100, 160), (40, 20000, 300)]
+          (2600, 2100, 160), (40, 20000, 300),
+          (400, 600, 1100), (1000, 900, 4000), (500, 2100, 2050), (255, 257, 16384)]
 
 
 @pytest.fixture(scope="module")
