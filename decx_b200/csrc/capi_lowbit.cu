@@ -251,7 +251,7 @@ bool q8_pair_split(uint64_t tiles, uint32_t n_kb) {
     static std::atomic<uint64_t> done{0};
     static std::atomic<int> held;
     auto kern = gemm_q8_pair_kernel<true, T>;
-    if (n_kb < 8 || tiles > 37 || allow_smem(kern, PairCfg::SMEM_BYTES, done) != 0) return false;
+    if (n_kb < 8 || allow_smem(kern, PairCfg::SMEM_BYTES, done) != 0) return false;
     return int64_t(tiles) <= clusters_at_once(kern, PairCfg::THREADS, PairCfg::SMEM_BYTES, 4, held);
 }
 

@@ -121,15 +121,15 @@ row_q8_kernel(const RowQ8Params p) {
     __shared__ uint32_t red_top[32];
     const uint32_t tpr = WARP ? 32u : blockDim.x;
     const uint32_t tid = WARP ? (threadIdx.x & 31u) : threadIdx.x;
-    const uint32_t row_step = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+    const uint64_t row_step = WARP ? uint64_t(gridDim.x) * (blockDim.x >> 5) : gridDim.x;
     griddep_launch();
     griddep_wait();
     const T* w = static_cast<const T*>(p.w);
-    for (uint32_t row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x; row < p.rows; row += row_step) {
-        const T* x = static_cast<const T*>(p.x) + uint64_t(row) * p.ldx;
-        const T* r = p.r != nullptr ? static_cast<const T*>(p.r) + uint64_t(row) * p.ldr : nullptr;
-        T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + uint64_t(row) * p.lds : nullptr;
-        uint8_t* q = p.q + uint64_t(row) * p.ldq;
+    for (uint64_t row = WARP ? uint64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x; row < p.rows; row += row_step) {
+        const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+        const T* r = p.r != nullptr ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
+        T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.lds : nullptr;
+        uint8_t* q = p.q + row * p.ldq;
         float v[NCH][8];
         float ss = 0.f;
         uint32_t top = 0;
@@ -226,8 +226,9 @@ row_q8_kernel(const RowQ8Params p) {
 // slot, so the ring needs no barrier; the only one per row is the reduction's.
 //
 // SHIFT: rows of x, r and sum that start anywhere (an odd row length).  The warps then copy the aligned units that their
-// elements touch (33 for 32 lanes), and a lane shifts what it needs out of two of them; on the way out the lanes pass
-// each other what an aligned unit of the other side needs.
+// elements touch (33 for 32 lanes), and the lanes take single elements, 32 neighbours at a time: that reads shared memory
+// without bank conflicts and writes whole segments whatever the alignment.  (Units shifted into place in registers and
+// passed between lanes took 85 instructions per element, and 180 us for 8192 x 4099 fp32 with a residual.)
 
 __device__ __forceinline__ void q8_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -238,25 +239,6 @@ __device__ __forceinline__ void q8_async_wait(uint32_t ahead) {
     if (ahead == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else if (ahead == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
-}
-
-// four words of `s` from byte `o` (below 16; whole words only when WORDS) on
-template <bool WORDS, int WS>
-__device__ __forceinline__ void q8_pick_at(const uint32_t (&s)[8], uint32_t o, uint32_t (&out)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (WORDS) out[i] = s[WS + i];
-        else out[i] = __funnelshift_r(s[WS + i], s[WS + i + 1], (o & 2) * 8);
-    }
-}
-template <bool WORDS>
-__device__ __forceinline__ void q8_pick(const uint32_t (&s)[8], uint32_t o, uint32_t (&out)[4]) {
-    switch (o >> 2) {                                     // the same for a whole row
-        case 0: q8_pick_at<WORDS, 0>(s, o, out); break;
-        case 1: q8_pick_at<WORDS, 1>(s, o, out); break;
-        case 2: q8_pick_at<WORDS, 2>(s, o, out); break;
-        default: q8_pick_at<WORDS, 3>(s, o, out); break;
-    }
 }
 
 // one 16-byte unit as floats and back
@@ -284,27 +266,6 @@ __device__ __forceinline__ void q8_words(const float (&f)[4], uint32_t* w) {
     for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
 }
 
-// One unit per lane, consecutive over the warp, to a row that starts anywhere; every lane's unit is whole.
-template <typename T, int E>
-__device__ __forceinline__ void q8_store_shift(T* at, const float (&f)[E], uint32_t lane) {
-    uint32_t s[8], out[4];
-    q8_words(f, s);
-    const uint32_t o = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
-    if (o == 0) {
-        *reinterpret_cast<uint4*>(at) = make_uint4(s[0], s[1], s[2], s[3]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[4 + i] = __shfl_down_sync(0xffffffffu, s[i], 1);
-    const uint32_t d = 16 - o, head = d / sizeof(T);      // the first aligned unit starts this many elements in
-    q8_pick<sizeof(T) == 4>(s, d, out);
-    if (lane < 31) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + d) = make_uint4(out[0], out[1], out[2], out[3]);
-    // what lies before the warp's first and behind its last aligned unit
-#pragma unroll
-    for (uint32_t i = 0; i < E; ++i)
-        if ((lane == 0 && i < head) || (lane == 31 && i >= head)) q8_store(at + i, f[i]);
-}
-
 // the larger of big, |a| and |b|; NaN if one of them is
 __device__ __forceinline__ void q8_max3(float& big, float a, float b) {
     asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(big) : "f"(a), "f"(b));
@@ -326,6 +287,12 @@ row_q8_ring_kernel(const RowQ8Params p) {
     const uint32_t unit_bytes = warps * WARP_BYTES, slot_bytes = unit_bytes * NC * MATS;
     const uint32_t mine = smem_u32(q8_ring) + wid * WARP_BYTES + lane * 16;
     const int32_t row_bytes = int32_t(p.cols * sizeof(T));
+    // column of element i of a thread's unit c.  SHIFT: lanes are neighbours, with one element each (fp32) or two (fp16: the
+    // pair's q bytes go out together)
+    auto column = [&](int c, int i) {
+        if (!SHIFT) return (c * tpr + tid) * E + i;
+        return (c * tpr + (tid & ~31u)) * E + (E == 4 ? i * 32 + lane : i / 2 * 64 + lane * 2 + i % 2);
+    };
     griddep_launch();
     griddep_wait();
 
@@ -334,15 +301,14 @@ row_q8_ring_kernel(const RowQ8Params p) {
     if constexpr (NORM) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint32_t col = (c * tpr + tid) * E;
-            const T* wp = static_cast<const T*>(p.w) + col;
-            if (col + E <= p.cols) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wp));
+            const T* const wp = static_cast<const T*>(p.w);
+            if (!SHIFT && column(c, E - 1) < p.cols) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wp + column(c, 0)));
                 w[c][0] = u.x; w[c][1] = u.y; w[c][2] = u.z; w[c][3] = u.w;
             } else {
                 float a[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) a[i] = col + i < p.cols ? q8_load(wp + i) : 0.f;
+                for (int i = 0; i < E; ++i) a[i] = column(c, i) < p.cols ? q8_load(wp + column(c, i)) : 0.f;
                 q8_words(a, w[c]);
             }
         }
@@ -388,20 +354,30 @@ row_q8_ring_kernel(const RowQ8Params p) {
         put += slot_bytes;
         if (put == p.depth * slot_bytes) put = 0;
     };
-    // this thread's elements of a unit; what lies behind the row's end is not zero
+    // this thread's elements of its unit at `src` (of a row that starts at byte `o` of its first unit); what lies behind the
+    // row's end is not zero
     auto take = [&](uint32_t src, uint32_t o, float (&f)[E]) {
-        uint32_t s[8], o4[4];
-        const uint4 v = ld_shared_v4(src);
-        s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w;
         if constexpr (SHIFT) {
-            const uint4 n = ld_shared_v4(src + 16);
-            s[4] = n.x; s[5] = n.y; s[6] = n.z; s[7] = n.w;
-            q8_pick<sizeof(T) == 4>(s, o, o4);
-        } else {
+            const T* const at = reinterpret_cast<const T*>(q8_ring + (src - smem_u32(q8_ring)) - lane * 16 + o) + lane * (E / 4);
+            if constexpr (E == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o4[i] = s[i];
+                for (int i = 0; i < E; ++i) f[i] = q8_load(at + i * 32);
+            } else if ((o & 2) == 0) {                                // the same for a whole row
+#pragma unroll
+                for (int i = 0; i < E; i += 2) {
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(at + i * 32));
+                    f[i] = a.x;
+                    f[i + 1] = a.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] = q8_load(at + i / 2 * 64 + i % 2);
+            }
+        } else {
+            const uint4 v = ld_shared_v4(src);
+            const uint32_t u4[4] = {v.x, v.y, v.z, v.w};
+            q8_unit(u4, f, T());
         }
-        q8_unit(o4, f, T());
     };
 
     for (uint32_t d = 0; d + 1 < p.depth; ++d) request_row();
@@ -419,8 +395,7 @@ row_q8_ring_kernel(const RowQ8Params p) {
         float ss = 0.f, big = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint32_t col = (c * tpr + tid) * E;
-            const bool all = col + E <= p.cols;
+            const bool all = column(c, E - 1) < p.cols;               // of this thread (columns grow with i)
             take(mine + get + c * unit_bytes, ox, v[c]);
             if constexpr (RES) {
                 float a[E];
@@ -431,20 +406,23 @@ row_q8_ring_kernel(const RowQ8Params p) {
             if (!all) {
 #pragma unroll
                 for (int i = 0; i < E; ++i)
-                    if (col + i >= p.cols) v[c][i] = 0.f;
+                    if (column(c, i) >= p.cols) v[c][i] = 0.f;
             }
             if constexpr (RES) {
                 if (sum != nullptr) {
-                    if (SHIFT && (c * tpr + (tid | 31u) + 1) * E <= p.cols) {          // the whole warp has whole units
-                        q8_store_shift<T, E>(sum + col, v[c], lane);
-                    } else if (!SHIFT && all) {
+                    if (!SHIFT && all) {
                         uint32_t o[4];
                         q8_words(v[c], o);
-                        *reinterpret_cast<uint4*>(sum + col) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(sum + column(c, 0)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    } else if (SHIFT && E == 8 && all && (reinterpret_cast<uintptr_t>(sum) & 2) == 0) {
+                        uint32_t o[4];
+                        q8_words(v[c], o);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(sum + column(c, 2 * i)) = o[i];
                     } else {
 #pragma unroll
                         for (int i = 0; i < E; ++i)
-                            if (col + i < p.cols) q8_store(sum + col + i, v[c][i]);
+                            if (all || column(c, i) < p.cols) q8_store(sum + column(c, i), v[c][i]);
                     }
                 }
             }
@@ -494,18 +472,21 @@ row_q8_ring_kernel(const RowQ8Params p) {
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const uint32_t col = (c * tpr + tid) * E;
             uint32_t o[E / 4];
 #pragma unroll
             for (int i = 0; i < E / 4; ++i)
                 o[i] = e4m3x2(v[c][4 * i] * mul, v[c][4 * i + 1] * mul) | (e4m3x2(v[c][4 * i + 2] * mul, v[c][4 * i + 3] * mul) << 16);
-            if (col + E <= p.cols) {
-                if constexpr (E == 8) *reinterpret_cast<uint2*>(q + col) = make_uint2(o[0], o[1]);
-                else *reinterpret_cast<uint32_t*>(q + col) = o[0];
+            const bool all = column(c, E - 1) < p.cols;
+            if (!SHIFT && all) {
+                if constexpr (E == 8) *reinterpret_cast<uint2*>(q + column(c, 0)) = make_uint2(o[0], o[1]);
+                else *reinterpret_cast<uint32_t*>(q + column(c, 0)) = o[0];
+            } else if (SHIFT && E == 8 && all) {
+#pragma unroll
+                for (int i = 0; i < E; i += 2) *reinterpret_cast<uint16_t*>(q + column(c, i)) = uint16_t(o[i / 4] >> (8 * (i & 3)));
             } else {
 #pragma unroll
                 for (int i = 0; i < E; ++i)
-                    if (col + i < p.cols) q[col + i] = uint8_t(o[i / 4] >> (8 * (i & 3)));
+                    if (all || column(c, i) < p.cols) q[column(c, i)] = uint8_t(o[i / 4] >> (8 * (i & 3)));
             }
         }
         q += uint64_t(step) * p.ldq;
@@ -522,11 +503,11 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(const RowQ8Params p) 
     const T* w = static_cast<const T*>(p.w);
     griddep_launch();
     griddep_wait();
-    for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* x = static_cast<const T*>(p.x) + uint64_t(row) * p.ldx;
-        const T* r = p.r != nullptr ? static_cast<const T*>(p.r) + uint64_t(row) * p.ldr : nullptr;
-        T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + uint64_t(row) * p.lds : nullptr;
-        uint8_t* q = p.q + uint64_t(row) * p.ldq;
+    for (uint64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+        const T* r = p.r != nullptr ? static_cast<const T*>(p.r) + row * p.ldr : nullptr;
+        T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.lds : nullptr;
+        uint8_t* q = p.q + row * p.ldq;
         float ss = 0.f;
         uint32_t top = 0;
         for (uint64_t k = threadIdx.x; k < p.cols; k += blockDim.x) {

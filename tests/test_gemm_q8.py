@@ -196,6 +196,75 @@ def test_quantised_layer(G, dev, tokens):
         assert torch.all((y4.double() - xq @ w4.t()).abs() <= tol)
 
 
+@gpu
+def test_first_calls_inside_a_capture():
+    """Nothing has to be called beforehand: in a fresh process, each operator's first call is a captured one."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = r"""
+import sys, torch
+sys.path.insert(0, %r)
+from decx_b200 import blas, gemm as G
+dev = torch.device("cuda:0")
+x, r = (torch.randn(24, 4096, device=dev).half() for _ in range(2))
+big = torch.randn(700, 2048, device=dev)
+w = torch.ones(4096, device=dev).half()
+W4 = blas.pack_q4(torch.randint(0, 16, (512, 4096), device=dev, dtype=torch.uint8))
+s4 = torch.rand(512, 64, device=dev).half()
+stream = torch.cuda.Stream()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    q, s, t = blas.rmsnorm_q8(x, w, residual=r)
+    y = blas.gemv_q4(W4, s4, q[:9], 64, x_scales=s[:9])
+    d = G.gemm_q8(q, s, q, s, out_dtype=torch.float32)
+    qb, sb = blas.cast_q8(big)
+    e = G.gemm_q8(qb, sb, qb, sb)
+graph.replay()
+torch.cuda.synchronize()
+q2, s2, t2 = blas.rmsnorm_q8(x, w, residual=r)
+y2 = blas.gemv_q4(W4, s4, q2[:9], 64, x_scales=s2[:9])
+d2 = G.gemm_q8(q2, s2, q2, s2, out_dtype=torch.float32)
+qb2, sb2 = blas.cast_q8(big)
+e2 = G.gemm_q8(qb2, sb2, qb2, sb2)
+torch.cuda.synchronize()
+print("SAME", torch.equal(t, t2), torch.equal(y, y2), torch.equal(d, d2), torch.equal(e, e2))
+""" % root
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "SAME True True True True" in run.stdout, run.stdout + run.stderr
+
+
+@gpu
+def test_calls_on_two_streams_at_once(G, dev):
+    """No workspace and no state between calls: two streams that overlap give what one after the other gives."""
+    from decx_b200 import blas
+    g = torch.Generator(device=dev).manual_seed(8)
+    x = [torch.randn(300, 2048, generator=g, device=dev).half() for _ in range(2)]
+    w = torch.ones(2048, dtype=torch.float16, device=dev)
+    B, sb = _operand(dev, g, 1536, 2048)
+    W4 = blas.pack_q4(torch.randint(0, 16, (2000, 2048), generator=g, device=dev, dtype=torch.uint8))
+    s4 = torch.rand(2000, 16, generator=g, device=dev).half()
+
+    def chain(v):
+        q, s, _ = blas.rmsnorm_q8(v, w)
+        return G.gemm_q8(q, s, B, sb), G.gemm_q8(q[:5], s[:5], B, sb), blas.gemv_q4(W4, s4, q[:3], 128, x_scales=s[:3])
+
+    want = [chain(v) for v in x]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(chain(x[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
 def test_refusals_of_the_c_abi():
     from decx_b200 import capi
     buf = (ctypes.c_float * 4096)()
