@@ -119,23 +119,27 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
     }
 }
 
-// `n` finished sums of tokens m0.. for column `col` (a lane's column: a warp writes 32 neighbouring elements of a row of D)
+// C of tokens m0 .. m0 + N - 1 in column `col` (a lane's column: a warp reads 32 neighbouring elements of a row).  Asked for
+// well before q8_thin_store needs it: these loads are what a small product with a C waits for.
 template <int N, typename T>
-__device__ __forceinline__ void q8_thin_store(const GemmQ8Params& p, uint32_t m0, uint32_t col, const float (&v)[N], const float* sa, float sbn) {
+__device__ __forceinline__ void q8_thin_c(const GemmQ8Params& p, uint32_t m0, uint32_t col, float (&c)[N]) {
     if (col >= p.N) return;
-    float d[N];
+    const T* at = static_cast<const T*>(p.C) + uint64_t(m0) * p.ldc + col;
 #pragma unroll
-    for (int j = 0; j < N; ++j) d[j] = v[j] * (sa[j] * sbn);
-    if (p.C != nullptr) {
-        const T* c = static_cast<const T*>(p.C) + uint64_t(m0) * p.ldc + col;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (m0 + j < p.M) d[j] = fmaf(p.beta, q8_to_f32(c[uint64_t(j) * p.ldc]), d[j]);
-    }
+    for (int j = 0; j < N; ++j) c[j] = m0 + j < p.M ? q8_to_f32(at[uint64_t(j) * p.ldc]) : 0.f;
+}
+// N finished sums of the same tokens and column
+template <int N, bool HASC, typename T>
+__device__ __forceinline__ void q8_thin_store(const GemmQ8Params& p, uint32_t m0, uint32_t col, const float (&v)[N], const float (&c)[N],
+                                              const float* sa, float sbn) {
+    if (col >= p.N) return;
     T* at = static_cast<T*>(p.D) + uint64_t(m0) * p.ldd + col;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-        if (m0 + j < p.M) q8_put(at + uint64_t(j) * p.ldd, d[j]);
+    for (int j = 0; j < N; ++j) {
+        float d = v[j] * (sa[j] * sbn);
+        if constexpr (HASC) d = fmaf(p.beta, c[j], d);
+        if (m0 + j < p.M) q8_put(at + uint64_t(j) * p.ldd, d);
+    }
 }
 
 // Sends this thread's sums (column `n` of the tile, all its tokens) to the ranks that finish them: inbox layout
@@ -157,35 +161,83 @@ __device__ __forceinline__ void q8_send(uint32_t taddr, uint32_t inbox, uint32_t
         }
     }
 }
-// Adds what has arrived, in rank order, and finishes this rank's tokens.
-template <int BN, int RANKS, typename T>
-__device__ __forceinline__ void q8_finish(const GemmQ8Params& p, const float* inbox, const float* sa, uint32_t rank, uint32_t n, uint32_t tm,
-                                          uint32_t col, float sbn) {
-    constexpr int TPO = BN / RANKS, U = TPO < 4 ? 2 : 4;
+// Waits for what the ranks send, adds it in rank order and finishes this rank's tokens.  Without a C they
+// go by twos or fours, so that the first stores leave early; with one, up to 16 at a time, so that as many loads are in flight.
+template <int BN, int RANKS, bool HASC, typename T>
+__device__ __forceinline__ bool q8_finish(const GemmQ8Params& p, const float* inbox, uint32_t bar, uint64_t limit, const float* sa, uint32_t rank,
+                                          uint32_t n, uint32_t tm, uint32_t col, float sbn) {
+    constexpr int TPO = BN / RANKS, U = TPO < 4 ? 2 : 4, NB = !HASC ? U : TPO < 16 ? TPO : 16;
+    const uint32_t m0 = tm * BN + rank * TPO;
+    float c[NB], next[NB];
+    if constexpr (HASC) q8_thin_c<NB, T>(p, m0, col, c);
+    if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar, 0, limit))) return false;
 #pragma unroll 1
-    for (int k = 0; k < TPO / U; ++k) {
-        float v[RANKS][U], s[U];
+    for (int b = 0; b < TPO / NB; ++b) {
+        if (m0 + b * NB >= p.M) break;
+        if constexpr (HASC) {
+            if (b + 1 < TPO / NB) q8_thin_c<NB, T>(p, m0 + (b + 1) * NB, col, next);
+        }
+        float s[NB];
 #pragma unroll
-        for (int r = 0; r < RANKS; ++r) {
-            const float* at = inbox + ((r * (TPO / U) + k) * 128 + n) * U;
-            if constexpr (U == 2) {
-                const float2 f = *reinterpret_cast<const float2*>(at);
-                v[r][0] = f.x; v[r][1] = f.y;
-            } else {
-                const float4 f = *reinterpret_cast<const float4*>(at);
-                v[r][0] = f.x; v[r][1] = f.y; v[r][2] = f.z; v[r][3] = f.w;
+        for (int k = 0; k < NB / U; ++k) {
+#pragma unroll
+            for (int e = 0; e < U; ++e) s[k * U + e] = 0.f;
+#pragma unroll
+            for (int r = 0; r < RANKS; ++r) {
+                const float* at = inbox + ((r * (TPO / U) + b * (NB / U) + k) * 128 + n) * U;
+                if constexpr (U == 2) {
+                    const float2 f = *reinterpret_cast<const float2*>(at);
+                    s[k * U] += f.x; s[k * U + 1] += f.y;
+                } else {
+                    const float4 f = *reinterpret_cast<const float4*>(at);
+                    s[k * U] += f.x; s[k * U + 1] += f.y; s[k * U + 2] += f.z; s[k * U + 3] += f.w;
+                }
             }
         }
+        q8_thin_store<NB, HASC, T>(p, m0 + b * NB, col, s, c, sa + rank * TPO + b * NB, sbn);
+        if constexpr (HASC) {
 #pragma unroll
-        for (int e = 0; e < U; ++e) {
-            s[e] = 0.f;
-#pragma unroll
-            for (int r = 0; r < RANKS; ++r) s[e] += v[r][e];
+            for (int j = 0; j < NB; ++j) c[j] = next[j];
         }
-        const uint32_t token = rank * TPO + k * U;
-        if (tm * BN + token >= p.M) break;
-        q8_thin_store<U, T>(p, tm * BN + token, col, s, sa + token, sbn);
     }
+    return true;
+}
+
+template <int BN, int RANKS, typename T>
+__device__ __forceinline__ bool q8_finish_c(const GemmQ8Params& p, const float* inbox, uint32_t bar, uint64_t limit, const float* sa, uint32_t rank,
+                                            uint32_t n, uint32_t tm, uint32_t col, float sbn) {
+    return p.C == nullptr ? q8_finish<BN, RANKS, false, T>(p, inbox, bar, limit, sa, rank, n, tm, col, sbn)
+                          : q8_finish<BN, RANKS, true, T>(p, inbox, bar, limit, sa, rank, n, tm, col, sbn);
+}
+// The tile whose K is not cut: the accumulator straight to D, up to 32 tokens at a time.
+template <int BN, bool HASC, typename T>
+__device__ __forceinline__ bool q8_direct(const GemmQ8Params& p, uint32_t bar, uint64_t limit, uint32_t taddr, uint32_t tm, uint32_t col,
+                                          const float* sa, float sbn) {
+    constexpr int CH = BN < 32 ? BN : 32;
+    float c[CH], next[CH];
+    if constexpr (HASC) q8_thin_c<CH, T>(p, tm * BN, col, c);
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar, 0, limit))) return false;
+    tc_fence_after_sync();
+#pragma unroll 1
+    for (uint32_t k = 0; k < BN / CH; ++k) {
+        const uint32_t m0 = tm * BN + k * CH;
+        if (m0 >= p.M) break;
+        if constexpr (HASC) {
+            if (k + 1 < BN / CH) q8_thin_c<CH, T>(p, m0 + CH, col, next);
+        }
+        uint32_t v[32];
+        tmem_ld_32x32(taddr + k * CH, v);
+        tmem_ld_wait();
+        float f[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) f[j] = __uint_as_float(v[j]);
+        q8_thin_store<CH, HASC, T>(p, m0, col, f, c, sa + k * CH, sbn);
+        if constexpr (HASC) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) c[j] = next[j];
+        }
+    }
+    return true;
 }
 
 template <int BN, bool SPLIT, typename T>
@@ -288,23 +340,15 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     float sbn = 0.f;
     if (warp >= 2) {
         sbn = col < p.N ? p.alpha * __ldg(p.sb + col) : 0.f;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
-        if (!ok && lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-        tc_fence_after_sync();
-        if (!split && ok) {
-            constexpr int CH = BN < 32 ? BN : 32;
-#pragma unroll 1
-            for (uint32_t c = 0; c < BN; c += CH) {
-                if (tm * BN + c >= p.M) break;
-                uint32_t v[32];
-                tmem_ld_32x32(tmem + ((quarter * 32u) << 16) + c, v);
-                tmem_ld_wait();
-                float f[CH];
-#pragma unroll
-                for (int j = 0; j < CH; ++j) f[j] = __uint_as_float(v[j]);
-                q8_thin_store<CH, T>(p, tm * BN + c, col, f, sa + c, sbn);
-            }
+        if (split) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
+            tc_fence_after_sync();
+        } else if (p.C == nullptr) {
+            ok = q8_direct<BN, false, T>(p, accf, limit, tmem + ((quarter * 32u) << 16), tm, col, sa, sbn);
+        } else {
+            ok = q8_direct<BN, true, T>(p, accf, limit, tmem + ((quarter * 32u) << 16), tm, col, sa, sbn);
         }
+        if (!ok && lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
     }
     if (split) {
         cluster_wait();                                               // every CTA of the cluster is there, its inbox ready
@@ -317,15 +361,10 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         __syncwarp();
         cluster_arrive();                                             // this CTA sends nothing more
         if (warp >= 2 && ok) {
-            if (!mbar_wait_cluster(inbar, 0, limit)) {
-                if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
-            } else if (p.ranks == 2) {
-                q8_finish<BN, 2, T>(p, inbox, sa, rank, n, tm, col, sbn);
-            } else if (p.ranks == 4) {
-                q8_finish<BN, 4, T>(p, inbox, sa, rank, n, tm, col, sbn);
-            } else {
-                q8_finish<BN, 8, T>(p, inbox, sa, rank, n, tm, col, sbn);
-            }
+            const bool got = p.ranks == 2   ? q8_finish_c<BN, 2, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
+                             : p.ranks == 4 ? q8_finish_c<BN, 4, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
+                                            : q8_finish_c<BN, 8, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn);
+            if (!got && lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
         }
         __syncwarp();
     }
