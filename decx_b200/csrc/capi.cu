@@ -108,24 +108,22 @@ int make_map(CUtensorMap* map, bool f16, const void* base, uint64_t rows, uint64
 
 }  // namespace
 
-// The same for another translation unit: bytes, fp16 or fp32, the swizzle as wide as the box (128 or 64 bytes).
+// The same for another translation unit: bytes, fp16 or fp32, the swizzle as wide as the box (128 or 64 bytes).  Encoded
+// anew for every call: such calls go through a model's many matrices, which would only push one another out of the cache.
 int dxb_host::tensor_map_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                             uint32_t box_cols, uint32_t box_rows) {
-    const CUtensorMapSwizzle swizzle = box_cols * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    if (elem_bytes != 1) return make_map(map, elem_bytes == 2, base, rows, cols, ld, box_cols, box_rows, swizzle);
-    const MapKey mk = {base, rows, cols, ld, box_cols, box_rows, 0, 2, int(swizzle), 2};
-    if (const CUtensorMap* hit = t_maps.find(mk)) { *map = *hit; ++t_map_hits; return 0; }
-    ++t_map_misses;
     EncodeTiledFn enc = encode_tiled_fn();
     if (enc == nullptr) return DECXB200_EDRIVER;
+    const CUtensorMapDataType type = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ld};
+    cuuint64_t strides[1] = {ld * uint64_t(elem_bytes)};
     cuuint32_t box[2] = {box_cols, box_rows};
     cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_SUCCESS) t_maps.put(mk, *map);
+    const CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           box_cols * elem_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : DECXB200_EDRIVER;
 }
 

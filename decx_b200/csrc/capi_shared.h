@@ -15,7 +15,7 @@ inline uint64_t round_up(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Tensor map of a pitched rows x cols matrix with a box_cols x box_rows box, zero fill; elements of 1 (bytes), 2 (fp16) or
-// 4 (fp32) bytes; swizzled within the box's width, 128 or 64 bytes.  Cached per thread.
+// 4 (fp32) bytes; swizzled within the box's width, 128 or 64 bytes.
 int tensor_map_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                   uint32_t box_cols, uint32_t box_rows);
 // how long a wait inside a kernel may last before it reports through the status word

@@ -89,6 +89,9 @@ struct ThinCfg {
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE + 1024 /*alignment slack*/ + 256 /*barriers*/ + BN * 4 /*scales of A*/ + INBOX;
     static constexpr uint32_t IDESC = umma_idesc(0u, false, false, 128, BN);
     static_assert(16 * STAGES + 24 <= 256, "barrier area");
+    // No CTA ever waits for tensor memory, whatever other kernels run: as many as shared memory admits leave enough of it,
+    // and a kernel that takes all of it takes more than half of the shared memory, too.
+    static_assert(228 * 1024 / (SMEM_BYTES + 1024) * TMEM_COLS <= 512 && SMEM_BYTES > 68 * 1024, "tensor memory for all CTAs of an SM");
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
