@@ -346,6 +346,7 @@ int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_t N, uint32_t
     if (d_dtype != DECXB200_FP16 && d_dtype != DECXB200_FP32) return DECXB200_EINVAL;
     if (A == nullptr || B == nullptr || D == nullptr || a_scales == nullptr || b_scales == nullptr) return DECXB200_EINVAL;
     if (M == 0 || N == 0 || K == 0 || lda < K || ldb < K || ldd < N || (C != nullptr && ldc < N)) return DECXB200_EINVAL;
+    if (C == D && ldc != ldd) return DECXB200_EINVAL;         // in place only element by element
     if (tile < DECXB200_TILE_AUTO || tile > DECXB200_TILE_Q8_PAIR) return DECXB200_EINVAL;
     if (M > 0x7fffff00u || N > 0x7fffff00u || K > 0x7fffff00u) return DECXB200_ETOOLARGE;   // TMA coordinates are signed
     if (!aligned16(A) || !aligned16(B) || (lda % 16) != 0 || (ldb % 16) != 0) return DECXB200_EALIGN;

@@ -215,13 +215,14 @@ PyObject* gemm_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         const float alpha = args[5] == Py_None ? 1.f : number(args[5]);
         const float beta = args[6] == Py_None || C == nullptr ? 0.f : number(args[6]);
-        const int tile = int(integer(args[9]));
+        const long tile = integer(args[9]);
         const uint64_t ldc = C != nullptr ? pitch(*C) : 0, ldd = pitch(D);
         return launch(A, [&](void* stream) {
             return decxb200_gemm_q8(type, stream, extent(M), extent(N), extent(K), A.data_ptr(), lda,
                                     static_cast<const float*>(sa.data_ptr()), B.data_ptr(), ldb,
                                     static_cast<const float*>(sb.data_ptr()), C ? C->data_ptr() : nullptr, ldc, D.data_ptr(), ldd,
-                                    &alpha, &beta, status ? static_cast<unsigned*>(status->data_ptr()) : nullptr, tile);
+                                    &alpha, &beta, status ? static_cast<unsigned*>(status->data_ptr()) : nullptr,
+                                    tile >= 0 && tile <= 0xFFFF ? int(tile) : -1);
         });
     });
 }
@@ -233,7 +234,8 @@ PyObject* gemv_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const TensorBase& W = tensor(args[0], "W");
         const TensorBase& s = tensor(args[1], "scales");
         const TensorBase& x = tensor(args[2], "x");
-        const long group = integer(args[3]);
+        const long asked = integer(args[3]);
+        const uint32_t group = asked > 0 && asked <= 128 ? uint32_t(asked) : 0u;     // 0: refused below
         const TensorBase* z = maybe(args[4], "zeros");
         const TensorBase* xs = maybe(args[5], "x_scales");
         const TensorBase& y = tensor(args[6], "out");
@@ -246,7 +248,7 @@ PyObject* gemv_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t vectors = single ? 1 : x.size(0), cols = single ? x.size(0) : x.size(1), rows = W.size(0);
         if (single && cols > 1 && x.stride(0) != 1) refuse(PyExc_ValueError, "x must be contiguous");
         const uint64_t ldx = single ? uint64_t(cols) : pitch(x), ldw = pitch(W), lds = pitch(s), ldz = z != nullptr ? pitch(*z) : 0;
-        const int64_t groups = group > 0 ? (cols + group - 1) / group : 0;
+        const int64_t groups = group != 0 ? (cols + group - 1) / group : 0;
         const char* const shapes = "W is rows x ceil(cols / 2), scales and zeros rows x ceil(cols / group), x vectors of cols entries";
         is_matrix(W, rows, (cols + 1) / 2, shapes);
         is_matrix(s, rows, groups, shapes);
@@ -264,7 +266,7 @@ PyObject* gemv_q4(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (z != nullptr) same_device(W, *z);
         if (xs != nullptr) same_device(W, *xs);
         return launch(W, [&](void* stream) {
-            return decxb200_gemv_q4(xt, yt, stream, extent(rows), extent(cols), extent(vectors), uint32_t(group > 0 ? group : 0), W.data_ptr(),
+            return decxb200_gemv_q4(xt, yt, stream, extent(rows), extent(cols), extent(vectors), group, W.data_ptr(),
                                     ldw, s.data_ptr(), lds, z ? z->data_ptr() : nullptr, ldz, x.data_ptr(), ldx,
                                     xs ? static_cast<const float*>(xs->data_ptr()) : nullptr, y.data_ptr(), ldy);
         });

@@ -1,4 +1,5 @@
 """The 8-bit GEMM against the definition in 64 bits, both of its kernels, and the operators of a quantised layer in a row."""
+import contextlib
 import ctypes
 
 import pytest
@@ -265,6 +266,55 @@ def test_calls_on_two_streams_at_once(G, dev):
             assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
 
 
+@gpu
+def test_a_captured_fork_and_join_replays(G, dev):
+    """One graph in which the norm's output goes two ways, to a GEMM and, on another stream, to a 4-bit product that a cast
+    and a GEMM then join: replayed on new inputs it gives what the calls give one after the other."""
+    from decx_b200 import blas
+    g = torch.Generator(device=dev).manual_seed(18)
+    x = torch.randn(12, 2048, generator=g, device=dev).half()
+    w = torch.rand(2048, generator=g, device=dev).half()
+    B, sb = _operand(dev, g, 640, 2048)
+    E, se = _operand(dev, g, 320, 2640)
+    W4 = blas.pack_q4(torch.randint(0, 16, (2000, 2048), generator=g, device=dev, dtype=torch.uint8))
+    s4 = torch.rand(2000, 16, generator=g, device=dev).half()
+    q, s = blas.new_q8(12, 2048, dev)
+    joined = torch.empty(12, 2640, dtype=torch.float16, device=dev)
+    q2, s2 = blas.new_q8(12, 2640, dev)
+    out = torch.empty(12, 320, dtype=torch.float16, device=dev)
+
+    def calls(fork, join):
+        blas.rmsnorm_q8(x, w, out=q, scales=s)
+        with fork():
+            blas.gemv_q4(W4, s4, q, 128, x_scales=s, out=joined[:, 640:])
+        G.gemm_q8(q, s, B, sb, out=joined[:, :640])
+        join()
+        blas.cast_q8(joined, out=q2, scales=s2)
+        G.gemm_q8(q2, s2, E, se, out=out)
+
+    side = torch.cuda.Stream()
+
+    def forked():
+        side.wait_stream(torch.cuda.current_stream())
+        return torch.cuda.stream(side)
+
+    calls(contextlib.nullcontext, lambda: None)              # the plain order
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(forked, lambda: torch.cuda.current_stream().wait_stream(side))
+    for k in range(8):
+        x.normal_(generator=g)
+        calls(contextlib.nullcontext, lambda: None)
+        want = [t.clone() for t in (q, s, joined, q2, s2, out)]
+        for t in (q, s, joined, q2, s2, out):
+            t.zero_()
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((q, s, joined, q2, s2, out), want):
+            assert torch.equal(a.float(), b.float()), k
+
+
 def test_refusals_of_the_c_abi():
     from decx_b200 import capi
     buf = (ctypes.c_float * 4096)()
@@ -278,6 +328,7 @@ def test_refusals_of_the_c_abi():
     assert call(A=None) == -1 and call(B=None) == -1 and call(D=None) == -1 and call(sa=None) == -1 and call(sb=None) == -1
     assert call(lda=16) == -1 and call(ldb=16) == -1 and call(ldd=7) == -1 and call(C=p, ldc=7) == -1
     assert call(tile=3) == -1 and call(tile=-1) == -1
+    assert call(C=p, ldc=16) == -1                           # C is D, with another pitch
     assert call(M=0x7fffffff) == -5
     assert call(A=p + 8) == -2 and call(B=p + 4) == -2 and call(lda=40) == -2 and call(ldb=33) == -2
     assert call(sa=p + 2) == -2 and call(sb=p + 1) == -2 and call(D=p + 1) == -2 and call(dt=capi.FP32, C=p + 2, ldc=8) == -2
@@ -311,5 +362,7 @@ def test_refusals_of_the_front_end_on_the_gpu(G, dev):
         G.gemm_q8(A, sa, B, sb, out=torch.zeros(4, 9, device=dev))
     with pytest.raises(ValueError):
         G.gemm_q8(A, sa, B, sb.cpu())
+    with pytest.raises(capi.DecxB200Error):
+        G.gemm_q8(A, sa, B, sb, tile=2 ** 32)
     with pytest.raises(capi.DecxB200Error):
         G.gemm_q8(A[:, :24].contiguous(), sa, B[:, :24].contiguous(), sb)

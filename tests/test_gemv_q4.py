@@ -207,3 +207,7 @@ def test_refusals_of_the_front_end_on_the_gpu(Bl, dev):
         Bl.gemv_q4(W, s, x, 16 * 3)
     with pytest.raises(capi.DecxB200Error):
         Bl.gemv_q4(W, s, torch.zeros(17, 32, device=dev).half(), 32)
+    with pytest.raises(ValueError):
+        Bl.gemv_q4(W, s, x, 2 ** 32 + 32)                    # would be 32 in 32 bits
+    with pytest.raises(ValueError):
+        Bl.gemv_q4(W, s, x, -32)
