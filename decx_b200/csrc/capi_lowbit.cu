@@ -99,21 +99,24 @@ int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
     return launch_cluster(kern, unsigned(want < have ? want : have), threads, row * p.depth, 1, s, p);
 }
 
-// kernels that keep one row per CTA or warp: few rows (no ring to fill), or operands that only single elements fit
+// Kernels that keep one row per CTA or warp: rows that do not fit a ring, or operands that only single elements fit (VEC false:
+// any alignment, and fewer columns than a warp has lanes).  The ring is the faster one wherever it works, from a single row
+// on (norm of 37 x 512 fp16 with a residual 2.0 against 2.6 us, 296 x 8192 3.7 against 5.4, 1184 x 8192 13.4 against 20.6).
 template <typename T, bool NORM, bool VEC>
 int launch_row_q8(cudaStream_t s, const RowQ8Params& p) {
-    if (p.cols <= 1024) {
-        const unsigned blocks = unsigned((uint64_t(p.rows) + 7) / 8);
-        if (p.cols <= 256) return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 1>, blocks, 256, 0, 1, s, p);
-        if (p.cols <= 512) return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 2>, blocks, 256, 0, 1, s, p);
-        return launch_cluster(row_q8_kernel<T, NORM, true, VEC, 4>, blocks, 256, 0, 1, s, p);
-    }
     const unsigned blocks = p.rows < 0x7fffffffu ? p.rows : 0x7fffffffu;
+    if (p.cols > 8 * 4 * 1024) return launch_cluster(row_q8_long_kernel<T, NORM>, blocks, 1024, 0, 1, s, p);
     const uint32_t chunks = (p.cols + 7) / 8;
     auto threads = [&](uint32_t nch) { return (chunks + 32 * nch - 1) / (32 * nch) * 32; };
-    if (p.cols > 8 * 4 * 1024) return launch_cluster(row_q8_long_kernel<T, NORM>, blocks, 1024, 0, 1, s, p);
-    if (chunks <= 1024 && p.rows <= 296) return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 1>, blocks, threads(1), 0, 1, s, p);
-    if (chunks <= 2048) return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 2>, blocks, threads(2), 0, 1, s, p);
+    if constexpr (!VEC) {
+        const unsigned warps = unsigned((uint64_t(p.rows) + 7) / 8);
+        if (p.cols <= 256) return launch_cluster(row_q8_kernel<T, NORM, true, false, 1>, warps, 256, 0, 1, s, p);
+        if (p.cols <= 512) return launch_cluster(row_q8_kernel<T, NORM, true, false, 2>, warps, 256, 0, 1, s, p);
+        if (p.cols <= 1024) return launch_cluster(row_q8_kernel<T, NORM, true, false, 4>, warps, 256, 0, 1, s, p);
+    }
+    if constexpr (!VEC || (NORM && sizeof(T) == 4)) {         // two slots of fp32 rows and residuals end at 12800 columns
+        if (chunks <= 2048) return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 2>, blocks, threads(2), 0, 1, s, p);
+    }
     return launch_cluster(row_q8_kernel<T, NORM, false, VEC, 4>, blocks, threads(4), 0, 1, s, p);
 }
 
@@ -136,8 +139,8 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     const bool out8 = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 && aligned16(p.w);
     // two slots of the ring have to fit: the limit is 1024 threads times two pieces of 8, or shared memory
     const uint64_t slot = uint64_t(p.cols + 511) / 512 * (rows16 ? 512 : 528) * e * (p.r != nullptr ? 2 : 1);
-    const bool ring = out8 && p.cols >= 16 && p.cols <= 16384 && 2 * slot <= 200 * 1024 && (p.rows > 296 || !rows16);
-    if (!ring) return rows16 && out8 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
+    const bool ring = out8 && p.cols >= 16 && p.cols <= 16384 && 2 * slot <= 200 * 1024;
+    if (!ring) return rows16 && out8 && p.cols >= 16 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
     if constexpr (NORM) {
         if (p.r != nullptr)
             return rows16 ? launch_row_q8_shape<T, true, true, false>(s, p) : launch_row_q8_shape<T, true, true, true>(s, p);
