@@ -234,9 +234,9 @@ int clusters_at_once(K kern, unsigned threads, unsigned smem, unsigned size, std
     return n;
 }
 
-// How many CTAs cut a tile's K in the thin kernel: as many as are on the GPU at once (up to 64 tokens, whose CTAs are short
-// and share their SMs, a quarter more: 64 x 4096 x 16384 takes 17 us so and 20 us with half as many), at least two stages
-// each
+// How many CTAs cut a tile's K in the thin kernel, at least two stages each: as many as are on the GPU at once; up to 64
+// tokens, whose CTAs are short and share their SMs, as many as two turns take (64 x 8192 x 8192 17.2 against 20.5 us, 16 x
+// 6144 x 4096 6.7 against 8.5, though 16 x 16384 x 4096 15.0 against 14.4; 128 x 8192 x 8192 would take 28.3 for 20.3)
 template <int BN, typename T>
 uint32_t q8_thin_ranks(uint64_t tiles, uint32_t n_kb) {
     static std::atomic<uint64_t> done{0};
@@ -246,7 +246,7 @@ uint32_t q8_thin_ranks(uint64_t tiles, uint32_t n_kb) {
     if (allow_smem(kern, Cfg::SMEM_BYTES, done) != 0) return 1;
     uint32_t ranks = 1;
     for (int i = 1; i < 4; ++i)
-        if (n_kb >= (2u << i) && int64_t(tiles) * (BN < 128 ? 4 : 5) <= 5 * int64_t(clusters_at_once(kern, 192, Cfg::SMEM_BYTES, 1u << i, held[i])))
+        if (n_kb >= (2u << i) && int64_t(tiles) * (BN < 128 ? 1 : 2) <= 2 * int64_t(clusters_at_once(kern, 192, Cfg::SMEM_BYTES, 1u << i, held[i])))
             ranks = 1u << i;
     return ranks;
 }

@@ -18,8 +18,8 @@
 //                  products are bound by reading B, so K is cut over a cluster of up to 8 CTAs until the GPU is full.
 //                  Each CTA then sends its partial sums into the shared memory of the CTA that finishes these tokens
 //                  (st.async, counted by an mbarrier there), which adds them in rank order: one launch, no workspace,
-//                  no atomics, and no barrier that everybody has to reach at the end.  16 tokens, 16384 x 4096: 14.4 us,
-//                  73 % of a copy's bandwidth; 4096 x 4096: 6.0 us, 43 %, since a product that short is the sum of its
+//                  no atomics, and no barrier that everybody has to reach at the end.  16 tokens, 16384 x 4096: 15.0 us,
+//                  70 % of a copy's bandwidth; 4096 x 4096: 6.0 us, 43 %, since a product that short is the sum of its
 //                  latencies (first load 1 us, ring, join 1.3 us).
 // Every wait is bounded: on time-out the role writes a code to *status and the kernel unwinds.
 #pragma once
