@@ -31,7 +31,7 @@ def _stale(target, sources):
 
 def build_kernels(force=False, verbose=False):
     out = os.path.join(CSRC, "libdecx_b200.so")
-    srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))]
+    srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh", ".h"))]
     srcs.append(os.path.join(ROOT, "include", "decx_b200.h"))
     if force or _stale(out, srcs):
         cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + [

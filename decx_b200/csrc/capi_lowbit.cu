@@ -9,6 +9,7 @@
 #include "gemm_q8.cuh"
 #include "gemv_q4.cuh"
 #include "rownorm_q8.cuh"
+#include "rownorm_q8_plan.h"
 
 using namespace dxb;
 using dxb_host::aligned16;
@@ -72,12 +73,11 @@ int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
 
 template <typename T, bool NORM, bool RES, bool WARP, bool SHIFT, int NCH>
 int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
-    constexpr uint32_t UNITS = NCH * 8 * sizeof(T) / 16 * (RES ? 2 : 1);
-    const uint32_t row = threads / 32 * (SHIFT ? 33 : 32) * 16 * UNITS;      // one slot of the ring
+    const uint32_t slot = q8_ring_slot(threads, SHIFT, NCH * 8 * sizeof(T) / 16 * (RES ? 2 : 1));
     auto kern = row_q8_ring_kernel<T, NORM, RES, WARP, SHIFT, NCH>;
     static std::atomic<uint64_t> done{0};
     static std::atomic<int> regs{0};
-    int rc = allow_smem(kern, 220 * 1024, done);
+    int rc = allow_smem(kern, Q8_RING_SMEM, done);
     if (rc != 0) return rc;
     int r = regs.load(std::memory_order_relaxed);
     if (r == 0) {
@@ -86,17 +86,11 @@ int launch_row_q8_ring(cudaStream_t s, RowQ8Params p, uint32_t threads) {
         if (e != cudaSuccess) return int(e);
         regs.store(r = a.numRegs, std::memory_order_relaxed);
     }
-    const uint32_t by_regs = 65536u / (uint32_t((r + 7) / 8 * 8) * threads), by_threads = 2048u / threads;
-    const uint32_t most = by_regs < by_threads ? by_regs : by_threads;
-    p.depth = 4;
-    auto fits = [&](uint32_t d) { return 225u * 1024 / (row * d + 2048); };
-    while (p.depth > 2 && fits(p.depth) < most) --p.depth;            // as many CTAs as registers and threads allow
-    while (p.depth < 4 && fits(p.depth) == 1 && row * (p.depth + 1) <= 220 * 1024) ++p.depth;
-    const uint32_t by_smem = fits(p.depth);
-    const uint32_t per_sm = by_smem < most ? by_smem : most;
+    const Q8RingPlan plan = q8_ring_plan(slot, threads, uint32_t(r));
+    p.depth = plan.depth;
     const uint64_t want = WARP ? (uint64_t(p.rows) + threads / 32 - 1) / (threads / 32) : p.rows;
-    const uint64_t have = uint64_t(sm_count()) * (per_sm ? per_sm : 1);
-    return launch_cluster(kern, unsigned(want < have ? want : have), threads, row * p.depth, 1, s, p);
+    const uint64_t have = uint64_t(sm_count()) * plan.per_sm;
+    return launch_cluster(kern, unsigned(want < have ? want : have), threads, slot * p.depth, 1, s, p);
 }
 
 // Kernels that keep one row per CTA or warp: rows that do not fit a ring, or operands that only single elements fit (VEC false:
@@ -139,7 +133,7 @@ int run_row_q8(cudaStream_t s, const RowQ8Params& p) {
     const bool out8 = (reinterpret_cast<uintptr_t>(p.q) & 7) == 0 && p.ldq % 8 == 0 && aligned16(p.w);
     // two slots of the ring have to fit: the limit is 1024 threads times two pieces of 8, or shared memory
     const uint64_t slot = uint64_t(p.cols + 511) / 512 * (rows16 ? 512 : 528) * e * (p.r != nullptr ? 2 : 1);
-    const bool ring = out8 && p.cols >= 16 && p.cols <= 16384 && 2 * slot <= 200 * 1024;
+    const bool ring = out8 && p.cols >= 16 && p.cols <= 16384 && 2 * slot <= Q8_RING_SLOTS;
     if (!ring) return rows16 && out8 && p.cols >= 16 ? launch_row_q8<T, NORM, true>(s, p) : launch_row_q8<T, NORM, false>(s, p);
     if constexpr (NORM) {
         if (p.r != nullptr)
