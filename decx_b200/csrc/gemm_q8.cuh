@@ -346,7 +346,7 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t quarter = warp & 3u, n = quarter * 32 + lane, col = tn * 128 + n;       // of an epilogue thread
     float sbn = 0.f;
     if (warp >= 2) {
-        sbn = col < p.N ? p.alpha * __ldg(p.sb + col) : 0.f;
+        sbn = col < p.N ? p.alpha * p.sb[col] : 0.f;
         if (split) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
             tc_fence_after_sync();
@@ -589,7 +589,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const float sa = row < p.M ? p.alpha * p.sa[row] : 0.f;
             // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more, and C
             const uint32_t sb_col = tn * 256 + threadIdx.x - 64;
-            const float sb_mine = sb_col < p.N ? __ldg(p.sb + sb_col) : 0.f;
+            const float sb_mine = sb_col < p.N ? p.sb[sb_col] : 0.f;
             if (ok && p.c_tma) {
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");     // buffers q, q + 1 are free
                 fetch_c(0);

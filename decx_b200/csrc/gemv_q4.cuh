@@ -124,15 +124,16 @@ __host__ __device__ constexpr uint32_t q4_swizzle(uint32_t r) {
     return UNITS == 8 ? ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1) : (r & 2) | ((r >> 2) & 1);
 }
 
-// BYTES consecutive bytes (1, 2, 4, 8 or 16) from a naturally aligned address, as words
+// BYTES consecutive bytes (1, 2, 4, 8 or 16) from a naturally aligned address, as words.  Ordinary loads: the kernel lives while
+// the one in front of it may still be writing x, so the read-only path is not open to it.
 template <int BYTES>
 __device__ __forceinline__ void q4_load_bytes(const void* p, uint32_t (&w)[(BYTES + 3) / 4]) {
     // volatile: a load asked for a tile ahead must not sink to where its value is used
-    if constexpr (BYTES == 1) asm volatile("{\n\t.reg .u16 t;\n\tld.global.nc.u8 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(w[0]) : "l"(p));
-    else if constexpr (BYTES == 2) asm volatile("{\n\t.reg .u16 t;\n\tld.global.nc.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(w[0]) : "l"(p));
-    else if constexpr (BYTES == 4) asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-    else if constexpr (BYTES == 8) asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-    else asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    if constexpr (BYTES == 1) asm volatile("{\n\t.reg .u16 t;\n\tld.global.u8 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(w[0]) : "l"(p));
+    else if constexpr (BYTES == 2) asm volatile("{\n\t.reg .u16 t;\n\tld.global.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(w[0]) : "l"(p));
+    else if constexpr (BYTES == 4) asm volatile("ld.global.b32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    else if constexpr (BYTES == 8) asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    else asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
 }
 
 // -(byte i of w): the byte becomes the low mantissa bits of 2^23
@@ -342,13 +343,11 @@ gemv_q4_kernel(const GemvQ4Params p) {
             xsum[gi][n][1] = s[1] * 0x1p-24f;
         }
 
-    auto store = [&](uint32_t block, uint32_t i, float s) {   // i = vector * R + row
+    auto scale_of = [&](uint32_t i) { return p.xs != nullptr ? p.xs[i / Cfg::R] : 1.f; };      // asked for before the sum is there
+    auto store = [&](uint32_t block, uint32_t i, float s, float xs) {   // i = vector * R + row
         const uint32_t v = i / Cfg::R, r = block * Cfg::R + i % Cfg::R, row = row0 + r;
-        if (r < n_tiles * TR && row < p.rows) {               // the last block may have fewer tiles
-            s *= 0x1p24f;
-            if (p.xs != nullptr) s *= __ldg(p.xs + v);
-            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row] = q4_out<OUT>(s);
-        }
+        if (r < n_tiles * TR && row < p.rows)                 // the last block may have fewer tiles
+            static_cast<OUT*>(p.y)[uint64_t(v) * p.ldy + row] = q4_out<OUT>(s * 0x1p24f * xs);
     };
     // A cluster joins several blocks at a time: its barrier has to wait for a CTA's outstanding memory accesses.
     const uint32_t block_sums = Cfg::R * p.n_vec, per_join = Cfg::JOIN / block_sums;
@@ -358,6 +357,8 @@ gemv_q4_kernel(const GemvQ4Params p) {
         const cg::cluster_group cluster = cg::this_cluster();
         float* const from = sums + ((b0 / per_join) & 1u) * Cfg::JOIN;
         for (uint32_t i = rank * blockDim.x + threadIdx.x; i < n * block_sums; i += ranks * blockDim.x) {
+            const uint32_t k = i / block_sums;
+            const float xs = scale_of(i - k * block_sums);
             float s = 0.f;
             for (uint32_t c0 = 0; c0 < ranks; c0 += 8) {
                 float d[8];                                   // requested together
@@ -366,8 +367,7 @@ gemv_q4_kernel(const GemvQ4Params p) {
 #pragma unroll
                 for (uint32_t c = 0; c < 8; ++c) s += d[c];
             }
-            const uint32_t k = i / block_sums;
-            store(b0 + k, i - k * block_sums, s);
+            store(b0 + k, i - k * block_sums, s, xs);
         }
     };
 
@@ -445,11 +445,12 @@ gemv_q4_kernel(const GemvQ4Params p) {
         float* const own = sums + ((b / per_join) & 1u) * Cfg::JOIN + in_join * block_sums;
         for (uint32_t i = threadIdx.x; i < block_sums; i += blockDim.x) {
             const float* at = parts + buf * warps * (Cfg::PART / 4) + i / Cfg::R * RS + i % Cfg::R;
+            const float xs = ranks > 1 ? 1.f : scale_of(i);
             float s = 0.f;
 #pragma unroll 4
             for (uint32_t w = 0; w < active; ++w) s += at[w * (Cfg::PART / 4)];
             if (ranks > 1) own[i] = s;
-            else store(b, i, s);
+            else store(b, i, s, xs);
         }
         if (ranks > 1 && (in_join + 1 == per_join || b + 1 == blocks))
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");

@@ -331,7 +331,7 @@ row_q8_ring_kernel(const RowQ8Params p) {
         for (int c = 0; c < NC; ++c) {
             const T* const wp = static_cast<const T*>(p.w);
             if (!SHIFT && column(c, E - 1) < p.cols) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(wp + column(c, 0)));
+                const uint4 u = *reinterpret_cast<const uint4*>(wp + column(c, 0));
                 w[c][0] = u.x; w[c][1] = u.y; w[c][2] = u.z; w[c][3] = u.w;
             } else {
                 float a[E];

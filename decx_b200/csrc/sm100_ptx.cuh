@@ -51,7 +51,8 @@ __device__ __forceinline__ uint32_t ld_acquire_sys(const unsigned* p) {
 // (at once when the kernel was launched without such a dependency).
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets a grid that programmatically depends on this one start its CTAs as soon as every CTA of this one has got here (and
-// there is room); its griddep_wait() still waits for this grid to end.
+// there is room); its griddep_wait() still waits for this grid to end.  Such a grid lives while its inputs are being written: it
+// reads them behind its wait, by ordinary loads only (no ld.global.nc, no __ldg).
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void st_release_sys(unsigned* p, unsigned v) {
     asm volatile("st.release.sys.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
