@@ -359,6 +359,7 @@ int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_t N, uint32_t
     p.sa = a_scales; p.sb = b_scales;
     p.alpha = alpha != nullptr ? *alpha : 1.f;
     p.beta = beta != nullptr ? *beta : 0.f;
+    p.wide = !q8_ordinary(p.alpha, Q8_ALPHA_REACH);
     p.C = p.beta != 0.f ? C : nullptr;
     p.ldc = ldc;
     p.D = D; p.ldd = ldd;

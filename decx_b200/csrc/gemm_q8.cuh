@@ -41,6 +41,7 @@ struct GemmQ8Params {
     uint32_t tiles_m, tiles_n;
     uint32_t group_m;          // pair kernel: height of the rasterisation groups, in tiles
     uint32_t ranks;            // thin kernel: CTAs that share a tile's K = cluster size
+    int wide;                  // alpha is not ordinary (q8_ordinary)
     unsigned* status;
     unsigned long long wait_limit_ns;
 };
@@ -81,6 +82,33 @@ __device__ __forceinline__ float q8_to_f32(float v) { return v; }
 __device__ __forceinline__ float q8_to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ void q8_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void q8_put(__half* p, float v) { *p = __float2half_rn(v); }
+
+// The epilogues multiply a sum by one fp32 factor, alpha and the two scales.  That is right as long as no product of them can
+// leave the fp32 range: scales of 2^-50 to 2^50 or zero, alpha of 2^-20 to 2^20.  A tile with others ("wide") is finished by a
+// plain loop in 64 bits; the epilogue warps agree on that while the tile is being multiplied.
+constexpr float Q8_REACH = 0x1p50f, Q8_ALPHA_REACH = 0x1p20f;
+__host__ __device__ __forceinline__ bool q8_ordinary(float s, float reach) {
+    return s == 0.f || (fabsf(s) <= reach && fabsf(s) >= 1.f / reach);
+}
+// a barrier of the epilogue's `THREADS` threads that also says whether `mine` holds in any of them
+template <int THREADS>
+__device__ __forceinline__ bool q8_any(bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(uint32_t(mine)), "n"(THREADS)
+        : "memory");
+    return any != 0;
+}
+// one element of D, if it exists, from its finished sum
+template <typename T>
+__device__ __forceinline__ void q8_put_wide(const GemmQ8Params& p, uint32_t row, uint32_t col, float v, float sa) {
+    if (row >= p.M || col >= p.N) return;
+    float d = float(double(v) * (double(p.alpha) * double(sa)) * double(p.sb[col]));
+    if (p.C != nullptr) d = fmaf(p.beta, q8_to_f32(static_cast<const T*>(p.C)[uint64_t(row) * p.ldc + col]), d);
+    q8_put(static_cast<T*>(p.D) + uint64_t(row) * p.ldd + col, d);
+}
 
 // =============================================================================================== thin kernel
 template <int BN, bool SPLIT>
@@ -247,6 +275,27 @@ __device__ __forceinline__ bool q8_direct(const GemmQ8Params& p, uint32_t bar, u
     return true;
 }
 
+// The same for a wide tile: this rank's tokens, column `col`, from the inbox or (K not cut) from the accumulator
+template <int BN, bool SPLIT, typename T>
+__device__ __forceinline__ void q8_thin_wide(const GemmQ8Params& p, const float* inbox, uint32_t taddr, const float* sa, uint32_t rank, uint32_t n,
+                                             uint32_t tm, uint32_t col) {
+    const uint32_t tokens = SPLIT ? BN / p.ranks : BN, u = tokens < 4 ? 2 : 4;
+#pragma unroll 1
+    for (uint32_t t = 0; t < tokens; ++t) {
+        float s = 0.f;
+        if constexpr (SPLIT) {
+#pragma unroll 1
+            for (uint32_t r = 0; r < p.ranks; ++r) s += inbox[((r * (tokens / u) + t / u) * 128 + n) * u + t % u];
+        } else {
+            uint32_t v;
+            tmem_ld_32x1(taddr + t, v);
+            tmem_ld_wait();
+            s = __uint_as_float(v);
+        }
+        q8_put_wide<T>(p, tm * BN + rank * tokens + t, col, s, sa[rank * tokens + t]);
+    }
+}
+
 template <int BN, bool SPLIT, typename T>
 __global__ void __launch_bounds__(192)
 gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmQ8Params p) {
@@ -345,11 +394,18 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     const uint32_t quarter = warp & 3u, n = quarter * 32 + lane, col = tn * 128 + n;       // of an epilogue thread
     float sbn = 0.f;
+    bool wide = false;
     if (warp >= 2) {
-        sbn = col < p.N ? p.alpha * p.sb[col] : 0.f;
+        sbn = col < p.N ? p.sb[col] : 0.f;
+        wide = q8_any<128>(p.wide || !q8_ordinary(sbn, Q8_REACH) || (threadIdx.x - 64 < BN && !q8_ordinary(sa[threadIdx.x - 64], Q8_REACH)));
+        sbn *= p.alpha;
         if (split) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
             tc_fence_after_sync();
+        } else if (wide) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf, 0, limit));
+            tc_fence_after_sync();
+            if (ok) q8_thin_wide<BN, SPLIT, T>(p, inbox, tmem + ((quarter * 32u) << 16), sa, 0, n, tm, col);
         } else if (p.C == nullptr) {
             ok = q8_direct<BN, false, T>(p, accf, limit, tmem + ((quarter * 32u) << 16), tm, col, sa, sbn);
         } else {
@@ -368,9 +424,15 @@ gemm_q8_thin_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         __syncwarp();
         cluster_arrive();                                             // this CTA sends nothing more
         if (warp >= 2 && ok) {
-            const bool got = p.ranks == 2   ? q8_finish_c<BN, 2, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
-                             : p.ranks == 4 ? q8_finish_c<BN, 4, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
-                                            : q8_finish_c<BN, 8, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn);
+            bool got;
+            if (wide) {
+                got = __all_sync(0xffffffffu, mbar_wait_cluster(inbar, 0, limit));
+                if (got) q8_thin_wide<BN, SPLIT, T>(p, inbox, 0, sa, rank, n, tm, col);
+            } else {
+                got = p.ranks == 2   ? q8_finish_c<BN, 2, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
+                      : p.ranks == 4 ? q8_finish_c<BN, 4, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn)
+                                     : q8_finish_c<BN, 8, T>(p, inbox, inbar, limit, sa, rank, n, tm, col, sbn);
+            }
             if (!got && lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
         }
         __syncwarp();
@@ -408,6 +470,19 @@ __device__ __forceinline__ void q8_tile_coords(uint32_t t, const GemmQ8Params& p
     const uint32_t rows = min(p.group_m, p.tiles_m - first), r = t - g * per_group;
     tm = first + r % rows;
     tn = r / rows;
+}
+
+// A thread's row of a wide tile, `count` columns from `col` on.  `in`: what the other pair sent (SPLIT)
+template <bool SPLIT, typename T>
+__device__ __forceinline__ void q8_pair_wide(const GemmQ8Params& p, uint32_t taddr, const float* in, uint32_t row, uint32_t col, uint32_t count,
+                                             float sa) {
+#pragma unroll 1
+    for (uint32_t c = 0; c < count; ++c) {
+        uint32_t v;
+        tmem_ld_32x1(taddr + c, v);
+        tmem_ld_wait();
+        q8_put_wide<T>(p, row, col + c, __uint_as_float(v) + (SPLIT ? in[c / 4 * 512 + c % 4] : 0.f), sa);
+    }
 }
 
 // SPLIT: two pairs (a cluster of four CTAs) share a tile, each half of K.  Pair r finishes columns [128 r, +128): the CTAs that
@@ -586,7 +661,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                 }
             };
-            const float sa = row < p.M ? p.alpha * p.sa[row] : 0.f;
+            const float sa_mine = row < p.M ? p.sa[row] : 0.f, sa = p.alpha * sa_mine;
             // while the tile is being multiplied: its scales of B, once nobody reads the previous tile's any more, and C
             const uint32_t sb_col = tn * 256 + threadIdx.x - 64;
             const float sb_mine = sb_col < p.N ? p.sb[sb_col] : 0.f;
@@ -597,7 +672,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             sb_tile[threadIdx.x - 64] = sb_mine;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const bool wide = q8_any<256>(p.wide || !q8_ordinary(sa_mine, Q8_REACH) || !q8_ordinary(sb_mine, Q8_REACH));
             const uint32_t a = it & 1u, aph = (it >> 1) & 1u;
             if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(accf + 8 * a, aph, limit))) {
                 if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
@@ -627,8 +702,28 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                 }
             }
+            if (wide && ok) {
 #pragma unroll 1
-            for (uint32_t c = 0; c < share / 32 && ok; ++c) {     // 32 columns at a time: one box of fp16, two of fp32
+                for (uint32_t i = 0; i < 2; ++i) {                    // boxes of C that are on their way
+                    const uint32_t b = (q + i) % Cfg::BUFS;
+                    if (!((asked >> b) & 1u)) continue;
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(cbar + 8 * b, (cphase >> b) & 1u, limit))) {
+                        if (lane == 0) q8_report(p, Q8_TIMEOUT_EPILOGUE);
+                        ok = false;
+                    }
+                    cphase ^= 1u << b;
+                    asked ^= 1u << b;
+                }
+                if (ok)
+                    q8_pair_wide<SPLIT, T>(p, tmem + a * 256 + col_in_tile + ((quarter * 32u) << 16),
+                                           reinterpret_cast<const float*>(smem) + (half * share / 4 * 128 + quarter * 32 + lane) * 4, row, box_col(0),
+                                           share, sa_mine);
+                for (uint32_t k = 0; k < BOXES; ++k) {                // its boxes keep their place
+                    if (lane == 0) bulk_commit_group();
+                }
+            }
+#pragma unroll 1
+            for (uint32_t c = 0; c < share / 32 && ok && !wide; ++c) {    // 32 columns at a time: one box of fp16, two of fp32
                 if (box_col(c * (32 / CW)) >= p.N) {
                     for (uint32_t k = 0; k < 32 / CW; ++k) {      // boxes that do not exist keep their place
                         if (lane == 0) bulk_commit_group();

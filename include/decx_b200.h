@@ -233,6 +233,7 @@ DECXB200_API int decxb200_cast2d(int kind, void* stream, uint32_t rows, uint32_t
  *   ldb bytes per row; a_scales: M, b_scales: N fp32 factors.  These are the operands decxb200_cast_q8 and
  *   decxb200_rmsnorm_q8 write.  C, D: M x N of d_dtype (DECXB200_FP16 or DECXB200_FP32); C may be NULL, or D itself
  *   with D's pitch.  alpha, beta: host pointers, NULL means 1 / 0; C is not read when beta == 0.
+ *   Scales and alpha may be of any magnitude: a product of them outside the fp32 range does no harm to a result inside it.
  *   Sums are fp32; an fp16 D is rounded once.  tcgen05 kind::f8f6f4; one launch, no workspace, the same result every
  *   time.  lda, ldb: multiples of 16, bases 16-byte aligned.  status as for decxb200_gemm.  Asynchronous on `stream`.
  *   tile: DECXB200_TILE_AUTO, or one of the kernels (tests and measurements): THIN cuts K over a cluster of CTAs and is
