@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from . import _front, capi
+from . import capi
 from .gemm import _ld
 
 _OUT = {(capi.FP32, 0): torch.float32, (capi.FP16, capi.ACCU_L1): torch.float32,
@@ -95,7 +95,7 @@ def cast_q8(src, out=None, scales=None):
     ``scales[r] = max|src[r]| / 448`` and ``q = e4m3(src / scales[:, None])``.  Launches on torch's current stream."""
     if out is None or scales is None:
         out, scales = _q8_out(src, out, scales)
-    code = _front.cast_q8(src, out, scales)
+    code = capi.front.cast_q8(src, out, scales)
     if code:
         capi.check(code)
     return out, scales
@@ -111,7 +111,7 @@ def rmsnorm_q8(x, weight, residual=None, eps=1e-6, out=None, scales=None, sum_ou
         out, scales = _q8_out(x, out, scales)
     if sum_out is None and residual is not None:
         sum_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    code = _front.rmsnorm_q8(x, weight, residual, eps, out, scales, sum_out)
+    code = capi.front.rmsnorm_q8(x, weight, residual, eps, out, scales, sum_out)
     if code:
         capi.check(code)
     return out, scales, sum_out
@@ -138,7 +138,7 @@ def gemv_q4(W, scales, x, group, zeros=None, x_scales=None, out_dtype=torch.floa
     if out is None:
         rows = W.shape[0]
         out = torch.empty(rows if x.dim() == 1 else (x.shape[0], rows), dtype=out_dtype, device=W.device)
-    code = _front.gemv_q4(W, scales, x, group, zeros, x_scales, out)
+    code = capi.front.gemv_q4(W, scales, x, group, zeros, x_scales, out)
     if code:
         capi.check(code)
     return out

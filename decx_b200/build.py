@@ -61,22 +61,41 @@ def build_host(force=False):
 
 
 FRONT = os.path.join(HERE, "front")
+FRONT_SO, FRONT_STAMP = os.path.join(HERE, "_front.so"), os.path.join(FRONT, "built_for.txt")
+
+
+def _front_stamp():
+    """What _front.so is built for: this Python, this torch and its C++ ABI."""
+    import sysconfig
+    import torch
+    return f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}\n"
+
+
+def front_stale():
+    if _stale(FRONT_SO, [os.path.join(FRONT, "front.cpp"), os.path.join(ROOT, "include", "decx_b200.h")]):
+        return True
+    if not os.path.exists(FRONT_STAMP):
+        return True
+    with open(FRONT_STAMP) as f:
+        return f.read() != _front_stamp()
 
 
 def build_front(force=False):
     """The Python entry of the low-precision operators (front/front.cpp): decx_b200/_front.so, against this torch."""
     import sysconfig
     import torch
-    out, src = os.path.join(HERE, "_front.so"), os.path.join(FRONT, "front.cpp")
+    out, src = FRONT_SO, os.path.join(FRONT, "front.cpp")
     tdir = os.path.dirname(torch.__file__)
-    if force or _stale(out, [src, os.path.join(ROOT, "include", "decx_b200.h")]):
+    if force or front_stale():
         cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DDECXB200_TORCH="{torch.__version__}"',
                "-I", sysconfig.get_paths()["include"], "-I", os.path.join(tdir, "include"),
                "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(CUDA_HOME, "include"),
                src, "-o", out, "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
                "-L", CSRC, "-ldecx_b200", "-Wl,-rpath,$ORIGIN/csrc"]
         subprocess.run(cmd, check=True, cwd=FRONT)
+        with open(FRONT_STAMP, "w") as f:
+            f.write(_front_stamp())
     return out
 
 

@@ -17,6 +17,26 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libdecx_b200.so")
 
 
+class _Front:
+    """The calls of ``decx_b200/_front.so`` (the low-precision operators, their tensors checked in C++).  It is built against one
+    torch and one Python, and loaded when the first of these calls is made: the other front ends need ctypes only."""
+
+    def __getattr__(self, name):
+        import torch
+        try:
+            from . import _front
+            if _front.built_for != str(torch.__version__):
+                raise ImportError(f"it was built for torch {_front.built_for}, this is {torch.__version__}")
+        except ImportError as e:
+            raise ImportError(f"decx_b200/_front.so cannot be used: build it with `python -m decx_b200.build` ({e})") from e
+        call = getattr(_front, name)
+        setattr(self, name, call)            # found without this function from now on
+        return call
+
+
+front = _Front()
+
+
 class DecxB200Error(RuntimeError):
     def __init__(self, code, what):
         super().__init__(f"decx_b200 error {code}: {what}")

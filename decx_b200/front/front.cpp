@@ -290,4 +290,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", "Checked calls of the low
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__front() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__front() {
+    PyObject* const m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddStringConstant(m, "built_for", DECXB200_TORCH) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

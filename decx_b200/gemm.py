@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from . import _front, capi
+from . import capi
 
 _DTYPES = {torch.float32: capi.FP32, torch.float16: capi.FP16, torch.complex64: capi.CPLXF,
            torch.float64: capi.FP64, torch.complex128: capi.CPLXD}
@@ -84,7 +84,7 @@ def gemm_q8(A, scale_a, B, scale_b, C=None, alpha=None, beta=None, out=None, out
     current stream of A's device; returns ``out`` (asynchronous)."""
     if out is None:
         out = torch.empty((A.shape[0], B.shape[0]), dtype=out_dtype if C is None else C.dtype, device=A.device)
-    code = _front.gemm_q8(A, scale_a, B, scale_b, C, alpha, beta, out, status, tile)
+    code = capi.front.gemm_q8(A, scale_a, B, scale_b, C, alpha, beta, out, status, tile)
     if code:
         capi.check(code)
     return out
