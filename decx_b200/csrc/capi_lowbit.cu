@@ -8,12 +8,13 @@
 #include "capi_shared.h"
 #include "gemm_q8.cuh"
 #include "gemv_q4.cuh"
+#include "per_device.h"
 #include "rownorm_q8.cuh"
 #include "rownorm_q8_plan.h"
 
 using namespace dxb;
 using dxb_host::aligned16;
-using dxb_host::round_up;
+using dxb_host::PerDevice;
 
 namespace {
 
@@ -21,6 +22,10 @@ int sm_count() {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
     return n;
+}
+int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
 }
 
 // Launch configuration with a cluster of CTAs.  All kernels here wait for the grids before them themselves
@@ -165,23 +170,24 @@ int launch_gemv_q4(cudaStream_t s, GemvQ4Params p) {
     constexpr uint32_t X = X8 ? 8 : 16;
     p.vec_x = reinterpret_cast<uintptr_t>(p.x) % X == 0 && p.ldx % 8 == 0;
     // clusters the GPU holds at once: the grid, since they stay and take turns over the blocks of rows
-    static std::atomic<int> held[Q4_MAX_RANKS][Cfg::WARPS];
-    int clusters = held[p.ranks - 1][warps - 1].load(std::memory_order_relaxed);
-    if (clusters == 0) {
-        cudaError_t e;
+    static PerDevice held[Q4_MAX_RANKS][Cfg::WARPS];
+    const int device = current_device();
+    cudaError_t e = cudaSuccess;
+    const int clusters = held[p.ranks - 1][warps - 1].get(device, [&] {
+        int n = 0;
         if (p.ranks == 1) {
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&clusters, kern, int(32 * warps), Cfg::smem(warps));
-            clusters *= sm_count();
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, int(32 * warps), Cfg::smem(warps));
+            n *= sm_count();
         } else {
             cudaLaunchConfig_t cfg;
             cudaLaunchAttribute attr[2];
             cluster_config(cfg, attr, p.ranks, 32 * warps, Cfg::smem(warps), p.ranks, s);
-            e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+            e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
         }
-        if (e != cudaSuccess) return int(e);
-        if (clusters < 1) return DECXB200_ETOOLARGE;
-        held[p.ranks - 1][warps - 1].store(clusters, std::memory_order_relaxed);
-    }
+        return e == cudaSuccess ? n : 0;
+    });
+    if (e != cudaSuccess) return int(e);
+    if (clusters < 1) return DECXB200_ETOOLARGE;
     const uint64_t tiles = (uint64_t(p.rows) + Cfg::TR - 1) / Cfg::TR;
     p.tiles = uint32_t((tiles + clusters - 1) / clusters);
     const uint64_t n = (tiles + p.tiles - 1) / p.tiles;
@@ -214,18 +220,17 @@ int run_gemv_q4_group(cudaStream_t s, bool x8, bool f32, const GemvQ4Params& p) 
 }
 
 // ------------------------------------------------------------------------------------------------ 8-bit GEMM
-// How many clusters of `size` CTAs of a kernel the GPU holds at once (asked once per kernel and size)
+// How many clusters of `size` CTAs of a kernel the GPU holds at once (0: it does not say)
 template <typename K>
-int clusters_at_once(K kern, unsigned threads, unsigned smem, unsigned size, std::atomic<int>& known) {
-    int n = known.load(std::memory_order_relaxed);
-    if (n == 0) {
+int clusters_at_once(K kern, unsigned threads, unsigned smem, unsigned size, PerDevice& known) {
+    const int device = current_device();
+    return known.get(device, [&] {
+        int n = 0;
         cudaLaunchConfig_t cfg;
         cudaLaunchAttribute attr[2];
         cluster_config(cfg, attr, size, threads, smem, size, nullptr);
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) n = -1;
-        known.store(n, std::memory_order_relaxed);
-    }
-    return n;
+        return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
+    });
 }
 
 // How many CTAs cut a tile's K in the thin kernel, at least two stages each: as many as are on the GPU at once; up to 64
@@ -234,7 +239,7 @@ int clusters_at_once(K kern, unsigned threads, unsigned smem, unsigned size, std
 template <int BN, typename T>
 uint32_t q8_thin_ranks(uint64_t tiles, uint32_t n_kb) {
     static std::atomic<uint64_t> done{0};
-    static std::atomic<int> held[4];
+    static PerDevice held[4];
     auto kern = gemm_q8_thin_kernel<BN, true, T>;
     using Cfg = ThinCfg<BN, true>;
     if (allow_smem(kern, Cfg::SMEM_BYTES, done) != 0) return 1;
@@ -248,7 +253,7 @@ uint32_t q8_thin_ranks(uint64_t tiles, uint32_t n_kb) {
 template <typename T>
 bool q8_pair_split(uint64_t tiles, uint32_t n_kb) {
     static std::atomic<uint64_t> done{0};
-    static std::atomic<int> held;
+    static PerDevice held;
     auto kern = gemm_q8_pair_kernel<true, T>;
     if (n_kb < 8 || allow_smem(kern, PairCfg::SMEM_BYTES, done) != 0) return false;
     return int64_t(tiles) <= clusters_at_once(kern, PairCfg::THREADS, PairCfg::SMEM_BYTES, 4, held);
@@ -322,8 +327,9 @@ int run_gemm_q8(cudaStream_t s, const GemmQ8Params& p, const void* A, uint64_t l
             const uint64_t tiles = (uint64_t(p.M) + 255) / 256 * ((uint64_t(p.N) + 255) / 256);
             const uint64_t thin_tiles = (uint64_t(p.M) + 127) / 128 * ((uint64_t(p.N) + 127) / 128);
             const uint64_t r = q8_pair_split<T>(tiles, uint32_t(n_kb)) ? 2 : 1, tr = q8_thin_ranks<128, T>(thin_tiles, uint32_t(n_kb));
-            const uint64_t pair = (tiles * r + 73) / 74 * (n_kb / r) * 700 + (r > 1 ? 12000 : 5000);
-            const uint64_t thin = (thin_tiles * tr + 147) / 148 * (n_kb / tr) * 700 + (tr > 1 ? 8500 : 3000);
+            const uint64_t sms = uint64_t(sm_count()), pairs = sms > 1 ? sms / 2 : 1;
+            const uint64_t pair = (tiles * r + pairs - 1) / pairs * (n_kb / r) * 700 + (r > 1 ? 12000 : 5000);
+            const uint64_t thin = (thin_tiles * tr + sms - 1) / sms * (n_kb / tr) * 700 + (tr > 1 ? 8500 : 3000);
             if (pair < thin) tile = DECXB200_TILE_Q8_PAIR;
         }
     }
