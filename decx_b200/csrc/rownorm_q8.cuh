@@ -10,9 +10,10 @@
 // The norm sees the 32-bit h, not the rounded sum that is stored.
 //
 // HBM bounds it: (3 e + 1) bytes per element with a residual, e + 1 without (e bytes per element of x), against six or so
-// operations.  Measured, share of a copy's 6456 GB/s: cast of 4096 x 16384 fp16 31.2 us, 100 %; norm with a residual of
-// 8192 x 4096 fp16 44.5 us, 82 %, fp32 73.4 us, 92 %; 16384 x 512 fp16 11.1 us, 82 %.  Rows that start anywhere are bound
-// by instructions: 8192 x 4099 fp16 72 us, 50 %, fp32 111 us, 61 %.  A single row is latency: 2.0 us for 4096 fp16.
+// operations.  Measured, share of a copy's 6456 GB/s: cast of 4096 x 16384 fp16 31.1 us, 100 %, in a short run, 33 to 35 in a long
+// one under the power limit; norm with a residual of 8192 x 4096 fp16 43.4 us, 84 %, fp32 72.7 us, 93 %; 16384 x 512 fp16
+// 11.1 us, 82 %.  Rows that start anywhere are bound by instructions, 83 per element in fp32 where aligned fp16 rows take 26:
+// 8192 x 4099 fp16 69 us, 53 %, fp32 107 us, 63 %.  A single row is latency: 1.9 us for 4096 fp16.
 //
 // The maximum is taken over the bit patterns of |h w| as unsigned integers, which orders NaN above infinity above
 // every finite value: a row that holds one (or whose sum of squares overflows) gets NaN for its scale and all its q.
@@ -102,41 +103,51 @@ __device__ __forceinline__ void q8_reduce(float& ss, uint32_t& top, float* red_s
     }
 }
 
-// The row's scale and the factors of its quotients: mul = 448 / max|v * pre|, and for the cast `low`, what mul's rounding left
-// out.  `pre` keeps rows of tiny and of huge values where no factor leaves the fp32 range.
-struct Q8Factors {
-    float scale, pre, mul, low;
-};
+// NaN or infinity in the row, or a sum of squares beyond fp32
 template <bool NORM>
-__device__ __forceinline__ Q8Factors q8_factors(const RowQ8Params& p, float ss, uint32_t top) {
-    const float big = __uint_as_float(top);
-    const float nan = __uint_as_float(0x7fffffffu);
-    const bool bad = top >= 0x7f800000u || (NORM && !(ss <= 3.402823466e38f));
-    const float rms = NORM ? rsqrtf(ss / float(p.cols) + p.eps) : 1.f;
-    Q8Factors f;
-    f.scale = bad ? nan : big * rms / E4M3_MAX;
-    f.pre = big < 0x1p-100f ? 0x1p100f : big > 0x1p100f ? 0x1p-100f : 1.f;
-    const float d = big * f.pre;
-    f.mul = bad ? nan : (top == 0 ? 0.f : E4M3_MAX / d);
-    f.low = fmaf(-f.mul, d, E4M3_MAX) * f.mul * (1.f / E4M3_MAX);    // the remainder, which is exact, by d
-    return f;
+__device__ __forceinline__ bool q8_bad(float ss, uint32_t top) {
+    return top >= 0x7f800000u || (NORM && !(ss <= 3.402823466e38f));
 }
-// What e4m3 rounds.  The norm's values come out of fp32 roundings, and one more product does them no harm.  The cast's are
-// given, often with 11 bits, and may lie half way between two e4m3 neighbours: with mul alone, whose own rounding moves every
-// quotient of a row the same way, 1700 of the 67 million elements of a 4096 x 16384 fp16 cast did not go to the even one.
-// The factor in two pieces leaves one fp32 rounding of the quotient (division by a divisor known in advance: Brisebarre,
-// Muller and Raina, IEEE Trans. Computers 53, 2004): rows of 16-byte units take two elements at a time and the time they took
-// before (4096 x 16384 fp16 31.2 us); unaligned ones, which instructions bound, 4 % more (515 x 4099 fp32 4.3 us).
+// The row's scale: for the one thread that stores it.
 template <bool NORM>
-__device__ __forceinline__ float q8_quotient(float v, const Q8Factors& f) {
-    return NORM ? v * f.mul : fmaf(v, f.mul, v * f.low);
+__device__ __forceinline__ float q8_scale(const RowQ8Params& p, float ss, uint32_t top) {
+    const float rms = NORM ? rsqrtf(ss / float(p.cols) + p.eps) : 1.f;
+    return q8_bad<NORM>(ss, top) ? __uint_as_float(0x7fffffffu) : __uint_as_float(top) * rms / E4M3_MAX;
 }
 
+// What e4m3 rounds is v * pre times mul, 448 / max|v * pre|; `pre` keeps rows of tiny and of huge values where mul does not leave
+// the fp32 range.  The norm's values come out of fp32 roundings, and mul's does them no more harm.  The cast's are given, often
+// with 11 bits, and may lie half way between two e4m3 neighbours, where mul's rounding, the same for a whole row, took all of
+// them to one side: 1700 of the 67 million elements of a 4096 x 16384 fp16 cast did not go to the even neighbour.
+// A half-way value m, at most 31/16 of its power of two, is what v * mul rounds to as long as mul's relative error is below
+// 2^-24 * 16/31, half a last place of m.  For the one row in four whose mul is not that good, `low` is what it lacks, and the
+// quotient is v * mul + v * low, rounded once (division by a divisor known in advance: Brisebarre, Muller and Raina, IEEE Trans.
+// Computers 53, 2004).  Both pieces for every row cost 1.4 % of a cast under the power limit.
+struct Q8Factors {
+    float pre, mul, low;
+};
 template <bool NORM>
+__device__ __forceinline__ Q8Factors q8_factors(float ss, uint32_t top) {
+    const float big = __uint_as_float(top), nan = __uint_as_float(0x7fffffffu);
+    Q8Factors f;
+    f.pre = big < 0x1p-100f ? 0x1p100f : big > 0x1p100f ? 0x1p-100f : 1.f;
+    const float d = big * f.pre;
+    f.mul = q8_bad<NORM>(ss, top) ? nan : top == 0 ? 0.f : E4M3_MAX / d;
+    f.low = 0.f;
+    if constexpr (!NORM) {
+        const float r = fmaf(-f.mul, d, E4M3_MAX);                   // exact: 448 times mul's relative error
+        if (fabsf(r) > E4M3_MAX * 0x1p-24f * 0.515f) f.low = r * f.mul * (1.f / E4M3_MAX);
+    }
+    return f;
+}
+__device__ __forceinline__ float q8_quotient(float v, const Q8Factors& f) {
+    return f.low == 0.f ? v * f.mul : fmaf(v, f.mul, v * f.low);
+}
+// two quotients as e4m3 bytes, by paired instructions; LOW: of a row that has a low
+template <bool LOW>
 __device__ __forceinline__ uint32_t q8_two(float a, float b, const Q8Factors& f) {
-    if constexpr (NORM) return e4m3x2(a * f.mul, b * f.mul);
-    const float2 v = make_float2(a, b);
-    const float2 t = __ffma2_rn(v, make_float2(f.mul, f.mul), __fmul2_rn(v, make_float2(f.low, f.low)));
+    const float2 v = make_float2(a, b), m = make_float2(f.mul, f.mul);
+    const float2 t = LOW ? __ffma2_rn(v, m, __fmul2_rn(v, make_float2(f.low, f.low))) : __fmul2_rn(v, m);
     return e4m3x2(t.x, t.y);
 }
 
@@ -224,13 +235,13 @@ row_q8_kernel(const RowQ8Params p) {
             for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
         }
         q8_reduce<WARP>(ss, top, red_ss, red_top);
-        const Q8Factors f = q8_factors<NORM>(p, ss, top);
-        if (tid == 0) p.scales[row] = f.scale;
+        const Q8Factors f = q8_factors<NORM>(ss, top);
+        if (tid == 0) p.scales[row] = q8_scale<NORM>(p, ss, top);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const uint32_t col = VEC ? (c * tpr + tid) * 8 : c * 8 * tpr + tid;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[c][i] = q8_quotient<NORM>(v[c][i] * f.pre, f);
+            for (int i = 0; i < 8; ++i) v[c][i] = q8_quotient(v[c][i] * f.pre, f);
             if (VEC && col + 8 <= p.cols) {
                 uint2 o;
                 o.x = e4m3x2(v[c][0], v[c][1]) | (e4m3x2(v[c][2], v[c][3]) << 16);
@@ -256,7 +267,7 @@ row_q8_kernel(const RowQ8Params p) {
 // SHIFT: rows of x, r and sum that start anywhere (an odd row length).  The warps then copy the aligned units that their
 // elements touch (33 for 32 lanes), and the lanes take single elements, 32 neighbours at a time: that reads shared memory
 // without bank conflicts and writes whole segments whatever the alignment.  (Units shifted into place in registers and
-// passed between lanes took 85 instructions per element, and 180 us for 8192 x 4099 fp32 with a residual; this takes 111.)
+// passed between lanes took 85 instructions per element, and 180 us for 8192 x 4099 fp32 with a residual; this takes 107.)
 
 __device__ __forceinline__ void q8_async16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -489,33 +500,37 @@ row_q8_ring_kernel(const RowQ8Params p) {
             }
             top = __reduce_max_sync(0xffffffffu, top);
         }
-        const Q8Factors f = q8_factors<NORM>(p, ss, top);
-        if (tid == 0) p.scales[row] = f.scale;
+        const Q8Factors f = q8_factors<NORM>(ss, top);
+        if (tid == 0) p.scales[row] = q8_scale<NORM>(p, ss, top);
         if (f.pre != 1.f) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int i = 0; i < E; ++i) v[c][i] *= f.pre;
         }
+        auto store = [&](auto two) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            uint32_t o[E / 4];
+            for (int c = 0; c < NC; ++c) {
+                uint32_t o[E / 4];
 #pragma unroll
-            for (int i = 0; i < E / 4; ++i)
-                o[i] = q8_two<NORM>(v[c][4 * i], v[c][4 * i + 1], f) | (q8_two<NORM>(v[c][4 * i + 2], v[c][4 * i + 3], f) << 16);
-            const bool all = column(c, E - 1) < p.cols;
-            if (!SHIFT && all) {
-                if constexpr (E == 8) *reinterpret_cast<uint2*>(q + column(c, 0)) = make_uint2(o[0], o[1]);
-                else *reinterpret_cast<uint32_t*>(q + column(c, 0)) = o[0];
-            } else if (SHIFT && E == 8 && all) {
+                for (int i = 0; i < E / 4; ++i)
+                    o[i] = two(v[c][4 * i], v[c][4 * i + 1]) | (two(v[c][4 * i + 2], v[c][4 * i + 3]) << 16);
+                const bool all = column(c, E - 1) < p.cols;
+                if (!SHIFT && all) {
+                    if constexpr (E == 8) *reinterpret_cast<uint2*>(q + column(c, 0)) = make_uint2(o[0], o[1]);
+                    else *reinterpret_cast<uint32_t*>(q + column(c, 0)) = o[0];
+                } else if (SHIFT && E == 8 && all) {
 #pragma unroll
-                for (int i = 0; i < E; i += 2) *reinterpret_cast<uint16_t*>(q + column(c, i)) = uint16_t(o[i / 4] >> (8 * (i & 3)));
-            } else {
+                    for (int i = 0; i < E; i += 2) *reinterpret_cast<uint16_t*>(q + column(c, i)) = uint16_t(o[i / 4] >> (8 * (i & 3)));
+                } else {
 #pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (all || column(c, i) < p.cols) q[column(c, i)] = uint8_t(o[i / 4] >> (8 * (i & 3)));
+                    for (int i = 0; i < E; ++i)
+                        if (all || column(c, i) < p.cols) q[column(c, i)] = uint8_t(o[i / 4] >> (8 * (i & 3)));
+                }
             }
-        }
+        };
+        if (NORM || f.low == 0.f) store([&](float a, float b) { return q8_two<false>(a, b, f); });
+        else store([&](float a, float b) { return q8_two<true>(a, b, f); });
         q += uint64_t(step) * p.ldq;
         if (RES && sum != nullptr) sum += uint64_t(step) * p.lds;
     }
@@ -547,8 +562,8 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(const RowQ8Params p) 
             top = max(top, __float_as_uint(h) & 0x7fffffffu);
         }
         q8_reduce<false>(ss, top, red_ss, red_top);
-        const Q8Factors f = q8_factors<NORM>(p, ss, top);
-        if (threadIdx.x == 0) p.scales[row] = f.scale;
+        const Q8Factors f = q8_factors<NORM>(ss, top);
+        if (threadIdx.x == 0) p.scales[row] = q8_scale<NORM>(p, ss, top);
         for (uint64_t k = threadIdx.x; k < p.cols; k += blockDim.x) {
             float h = q8_load(x + k);
             if (NORM && r != nullptr) {
@@ -556,7 +571,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(const RowQ8Params p) 
                 if (sum != nullptr) q8_store(sum + k, h);
             }
             if (NORM) h *= q8_load(w + k);
-            q[k] = uint8_t(e4m3x2(q8_quotient<NORM>(h * f.pre, f), 0.f));
+            q[k] = uint8_t(e4m3x2(q8_quotient(h * f.pre, f), 0.f));
         }
     }
 }

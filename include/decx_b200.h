@@ -261,8 +261,10 @@ DECXB200_API int decxb200_gemm_q8(int d_dtype, void* stream, uint32_t M, uint32_
  *   norm sees h before it is rounded.  residual == NULL: nothing is added (sum must then be NULL); sum == NULL: the sum
  *   is not stored.  sum may be x or residual (the same pointer and pitch); otherwise inputs and outputs may not overlap.
  *   weight: cols elements.  eps: a positive normal fp32 number.
- *   decxb200_cast_q8 rounds the quotient src * 448 / max|src| to fp32 once and then to e4m3: ties between two e4m3 values
- *   go to the even one.  (The norm multiplies by a rounded 448 / max: a value within 2^-22 of a tie, relatively, may go either way.)
+ *   decxb200_cast_q8: a value half way between two multiples of the scale that e4m3 has neighbouring codes for goes to the
+ *   even one, whatever the row's maximum is; src with up to 11 significant bits is always rounded to the nearest.  Otherwise,
+ *   and for the norm, fp32 arithmetic in front of the rounding may take a value within 2^-22 of half way, relatively, to
+ *   either side.
  *   A row of zeros has scale 0 and q 0.  A row that holds a NaN or an infinity, or whose sum of squares exceeds the
  *   fp32 range, gets NaN for its scale and for every q.
  *   Any alignment and pitch works; 16-byte aligned bases (8-byte for q) and pitches are faster, and q needs a 16-byte
