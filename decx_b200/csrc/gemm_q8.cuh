@@ -9,7 +9,7 @@
 //                  that one tile's epilogue runs under the next tile's MMAs.  The pair form halves what each SM's shared
 //                  memory has to deliver per MMA: each CTA holds its own 128 rows of A and of B only.  What bounds it is
 //                  that memory: 64 bytes per clock read by the MMAs and 64 written by TMA at the full rate.  One 128 of K
-//                  takes 660 clocks in a long run, 512 at that rate.  (256 x 512 tiles, two accumulators sharing A, were
+//                  takes 630 to 660 clocks of a run, 512 at that rate (4096 x 8192 x 8192: 626, tensor pipe 82 % busy).  (256 x 512 tiles, two accumulators sharing A, were
 //                  measured: 2048 x 16384 x 4096 118 us against 102, 2048 x 4096 x 16384 99 against 102.)  8192 x 8192 x
 //                  8192: 375 us, 2.9 PFLOP/s, in a short run, 437 to 460 in a long one under the power limit.  Few tiles (512 x
 //                  8192 x 4096, 18.5 us, 1.86 PFLOP/s) add what is paid once: 2 us until the first MMA, 2.5 for the epilogue.
@@ -18,9 +18,11 @@
 //                  products are bound by reading B, so K is cut over a cluster of up to 8 CTAs until the GPU is full.
 //                  Each CTA then sends its partial sums into the shared memory of the CTA that finishes these tokens
 //                  (st.async, counted by an mbarrier there), which adds them in rank order: one launch, no workspace,
-//                  no atomics, and no barrier that everybody has to reach at the end.  16 tokens, 16384 x 4096: 15.0 us,
-//                  70 % of a copy's bandwidth; 4096 x 4096: 6.0 us, 43 %, since a product that short is the sum of its
-//                  latencies (first load 1 us, ring, join 1.3 us).
+//                  no atomics, and no barrier between the last partial sum and the tokens that wait for it (one at the very
+//                  end keeps the shared memory that is sent to alive).  16 tokens, 16384 x 4096: 15.0 us, 70 % of a copy's
+//                  bandwidth; 4096 x 4096: 6.0 us, 43 %, since a product that short is the sum of its latencies (first load
+//                  1 us, ring, join 1.3 us).
+// Sums are fp32 in the tensor path, whose adder truncates: up to 2^-23 of the running sum for every 32 products.
 // Every wait is bounded: on time-out the role writes a code to *status and the kernel unwinds.
 #pragma once
 #include <cuda_fp16.h>

@@ -27,11 +27,15 @@
 // that the instruction gives columns 2t, 2t+1, 2t+8, 2t+9 holds words t*w .. t*w+w-1 (w = 1 / 2 / 4, one shared-memory
 // load), and its registers hold the matching x as 0 4 2 6 1 5 3 7 within eight.
 //
-// Measured (16384 x 16384, fp16 x and y, share of a copy's 6456 GB/s): one vector 31.8 us with groups of 128, 68 %, and 49.4
-// with groups of 32 and zero points, 50 %; eight vectors 36.5 us, 59 %.  The issue of instructions bounds it: 236 for a
-// tile of 16 x 256 with groups of 128, 482 with groups of 32 and zero points (a scale, a zero point and a sum of x per
-// group and row).  Nine to sixteen vectors halve a warp's columns, for the registers of x, and so double the partial
-// sums: 4096 x 4096 7.9 us for 16 against 5.1 for 8.  Small products wait for latencies: 1024 x 1024 2.3 us.
+// A weight that is its group's zero point therefore adds no exact zero, but the rounding of two sums that cancel.
+//
+// Measured (16384 x 16384, fp16 x and y, share of a copy's 6456 GB/s): one vector 31.6 us with groups of 128, 68 %, and 48.9
+// with groups of 32 and zero points, 50 %; eight vectors 36.3 us, 59 %.  What bounds it is the length of a warp's chains (word,
+// mask, product, scale) with four warps per scheduler, all that the registers of x leave room for: 222 instructions for a tile
+// of 16 x 256 with groups of 128 are issued at 2.0 of 4 per clock, 461 with groups of 32 and zero points (a scale, a zero point
+// and a sum of x per group and row) at 2.7; the tensor path is busy for 30 and 19 %, DRAM for 47 and 37.  Clusters of four CTAs
+// leave 20 of the 148 SMs without one.  Nine to sixteen vectors halve a warp's columns, for the registers of x, and so double
+// the partial sums: 4096 x 4096 7.8 us for 16 against 4.9 for 8.  Small products wait for latencies: 1024 x 1024 2.2 us.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
