@@ -25,8 +25,9 @@ class _Front:
         import torch
         try:
             from . import _front
-            if _front.built_for != str(torch.__version__):
-                raise ImportError(f"it was built for torch {_front.built_for}, this is {torch.__version__}")
+            built_for = getattr(_front, "built_for", "an unknown version")
+            if built_for != str(torch.__version__):
+                raise ImportError(f"it was built for torch {built_for}, this is {torch.__version__}")
         except ImportError as e:
             raise ImportError(f"decx_b200/_front.so cannot be used: build it with `python -m decx_b200.build` ({e})") from e
         call = getattr(_front, name)

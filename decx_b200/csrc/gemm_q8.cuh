@@ -290,6 +290,7 @@ __device__ __forceinline__ void q8_thin_wide(const GemmQ8Params& p, const float*
             for (uint32_t r = 0; r < p.ranks; ++r) s += inbox[((r * (tokens / u) + t / u) * 128 + n) * u + t % u];
         } else {
             uint32_t v;
+            __syncwarp();                                             // lanes without a column are back
             tmem_ld_32x1(taddr + t, v);
             tmem_ld_wait();
             s = __uint_as_float(v);
@@ -481,6 +482,7 @@ __device__ __forceinline__ void q8_pair_wide(const GemmQ8Params& p, uint32_t tad
 #pragma unroll 1
     for (uint32_t c = 0; c < count; ++c) {
         uint32_t v;
+        __syncwarp();                                                 // lanes without a row are back
         tmem_ld_32x1(taddr + c, v);
         tmem_ld_wait();
         q8_put_wide<T>(p, row, col + c, __uint_as_float(v) + (SPLIT ? in[c / 4 * 512 + c % 4] : 0.f), sa);
@@ -716,6 +718,7 @@ gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     cphase ^= 1u << b;
                     asked ^= 1u << b;
                 }
+                __syncwarp();
                 if (ok)
                     q8_pair_wide<SPLIT, T>(p, tmem + a * 256 + col_in_tile + ((quarter * 32u) << 16),
                                            reinterpret_cast<const float*>(smem) + (half * share / 4 * 128 + quarter * 32 + lane) * 4, row, box_col(0),
